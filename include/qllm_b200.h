@@ -451,6 +451,87 @@ int qllm_k_attention(uint32_t encoding, const uint8_t* const* page_table, size_t
                      uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
                      uint32_t split_tokens, uint32_t max_splits, int bf16, void* workspace,
                      float* out, int impl, void* stream);
+/* ---- operators for batches of sequences over the paged cache -----------------------------------
+ * The provider decodes one stream; a host that batches streams calls these per layer, for all its
+ * sequences at once: the cache's writer, its reader, and its trimming by attention weight.  The
+ * cache is the one of the calls above (same pages, same records), one page table per sequence.
+ *
+ * All pointers are device memory of the current device unless stated, 4-byte aligned unless a call
+ * asks for more; the calls only enqueue on `stream`, allocate nothing, can be captured into a graph,
+ * and keep nothing in the library, so calls on several streams and threads may run at once as long as
+ * they share no workspace and no output.  Graphs that share a workspace must not run at once.
+ * Results do not depend on scheduling: the same inputs give the same bits on the same GPU model.
+ *
+ * qllm_kv_batch (host memory, read during the call).  page_tables [sequences, pages_per_sequence]:
+ * device pointers to pages; slot t of sequence s lies in page t / page_tokens of its row.  A page
+ * pointer that is null or not on a 16-byte boundary stands for no page: nothing is stored there, and
+ * its slots count as absent when the cache is read.  page_tokens: a multiple of 16; layer_offset: a
+ * multiple of 16, where the layer's records begin in a page; head_dim 64, 128, 192 or 256. */
+enum { QLLM_ROW_F32 = 0, QLLM_ROW_BF16 = 1, QLLM_ROW_F16 = 2 };
+#define QLLM_PADDING_SLOT 0xFFFFFFFFu
+typedef struct qllm_kv_batch {
+  uint8_t* const* page_tables;
+  size_t layer_offset;
+  uint32_t sequences, pages_per_sequence; /* at most 65535; below 2^31 slots per sequence */
+  uint32_t page_tokens, encoding;         /* QLLM_KV_* */
+  uint32_t kv_heads, head_dim;
+} qllm_kv_batch;
+/* Per-head RMS norm of queries and keys, rotation by position, and the K/V records
+ * (gated_gqa_qkv_rope_paged_batch_kernel with its per-head norm, transformer_kernels.cu:3551-3643,
+ * for rows of many sequences).  Row r of qkv [rows, (q_heads + 2 kv_heads) * head_dim] (row_type values,
+ * qkv_stride elements apart):
+ *   n = x * w / sqrt(mean(x^2) + eps) per query head (w = q_norm) and key head (w = k_norm), [head_dim] FP32;
+ *   the first rotary_dim values (a multiple of 16, may be 0) are rotated in pairs (i, i + rotary_dim / 2)
+ *   by positions[r] * inv_freq[i], the angle reduced in FP64;
+ *   query [rows, q_heads * head_dim], and key [rows, kv_heads * head_dim] unless it is null, get the
+ *   results in row_type; the K record (and the V record of the untouched value head) is made of the FP32
+ *   results, so every output is rounded once.  A quantised record's scale is max|v| / 127 (Q8) or / 7
+ *   (Q4H) as F16, at least 2^-24 and at most 65504; a NaN becomes code 0.
+ * The record of row r goes to slot row_slot[r] of sequence row_sequence[r] (null: sequence r); a
+ * sequence or slot outside the cache stores nothing.  row_slot null: no records at all (page_tables may
+ * be null).  A row whose slot is QLLM_PADDING_SLOT is left alone: none of its outputs are written.
+ * Two rows of one call must not name the same slot (its record would be a mixture of both).
+ * slot_positions [sequences, kv_heads, slot_stride] (optional): positions[r] is written for each
+ * head of the slot stored, which is what qllm_k_kv_evict reads.
+ * Rows and strides in multiples of 16 bytes.  query may be qkv itself, and key its key heads, with the
+ * same stride (in place). */
+int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, const void* qkv, size_t qkv_stride,
+                              uint32_t rows, uint32_t q_heads, uint32_t rotary_dim, const float* q_norm,
+                              const float* k_norm, float eps, const float* inv_freq, const uint32_t* positions,
+                              const uint32_t* row_sequence, const uint32_t* row_slot, void* query, size_t query_stride,
+                              void* key, size_t key_stride, uint32_t* slot_positions, size_t slot_stride,
+                              void* stream);
+/* Attention of one new token per sequence over its first lengths[s] slots (at most its capacity; the
+ * caller has stored the new token's own record):
+ *   z_t = scale * q . K_t;  p = softmax(z);  out = sum_t p_t V_t        per query head
+ *   weights_out[s, h, t] = weights_in[s, h, t] + sum of p_t over the query heads of kv head h
+ * query, out [sequences, q_heads * head_dim] of row_type, rows and strides in multiples of 16 bytes, not
+ * overlapping; scores, softmax statistics and sums are FP32, the result is rounded once.  A sequence of
+ * length 0 (or whose slots are all absent, or all score -inf) gives zeros.  weights_out
+ * [sequences, kv_heads, weights_stride] is optional; weights_in null: zeros; weights_in == weights_out: in
+ * place; slots at and behind lengths[s] are left alone.  workspace: at least
+ * qllm_k_decode_attention_workspace_bytes bytes on a 16-byte boundary, its content does not matter. */
+size_t qllm_k_decode_attention_workspace_bytes(const qllm_kv_batch* cache, uint32_t q_heads, int weights);
+int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const void* query, size_t query_stride,
+                            const uint32_t* lengths, uint32_t q_heads, float scale, const float* weights_in,
+                            float* weights_out, size_t weights_stride, void* out, size_t out_stride, void* workspace,
+                            size_t workspace_bytes, void* stream);
+/* Trims every sequence to `budget` slots per kv head by accumulated attention weight.  Of the
+ * n = lengths_in[s] slots (weights_in, positions_in [sequences, kv_heads, stride]) m = min(n, budget) are
+ * kept: first those whose position is among the last `recent` before next_positions[s]
+ * (position + recent >= next) or below `sinks`, then those of larger weight (NaN counts as -inf, -0 as
+ * 0), ties to the lower slot; recent + sinks <= budget.  Kept slots below m stay; the i-th freed slot
+ * below m takes record, weight and position of the i-th kept slot at or above m (both in slot order), so
+ * the records move in place and as few as possible.  weights_out and positions_out (== the inputs: in
+ * place) hold the kept slots' values at t < m, weights_out is zero for m <= t < n (a slot stored there
+ * later starts from nothing), everything else is left alone; lengths_out[s] = m (== lengths_in: in
+ * place).  Slots on absent pages move no record. */
+size_t qllm_k_kv_evict_workspace_bytes(const qllm_kv_batch* cache, uint32_t budget);
+int qllm_k_kv_evict(const qllm_kv_batch* cache, const uint32_t* lengths_in, uint32_t* lengths_out,
+                    const uint32_t* next_positions, uint32_t budget, uint32_t recent, uint32_t sinks,
+                    const float* weights_in, float* weights_out, const uint32_t* positions_in, uint32_t* positions_out,
+                    size_t stride, void* workspace, size_t workspace_bytes, void* stream);
+
 /* argmax_batch / topk_logits (transformer_kernels.cu:7059-7178) */
 int qllm_k_argmax(const float* values, uint32_t rows, uint32_t count, uint32_t row_stride,
                   uint32_t* out, void* stream);

@@ -1,0 +1,165 @@
+// extern "C" forms of the operators for batches of sequences (include/qllm_b200.h): every argument
+// that the host can see is checked here, before any CUDA call.
+#include <cmath>
+#include <string>
+
+#include "kv_batch.cuh"
+
+using namespace qllm;
+
+namespace {
+
+bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1U)) == 0U; }
+
+// Whether [p, p + bytes) and [q, q + bytes_q) share memory.
+bool overlap(const void* p, size_t bytes, const void* q, size_t bytes_q) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a < b + bytes_q && b < a + bytes;
+}
+
+size_t row_bytes(uint32_t type) { return type == QLLM_ROW_F32 ? 4U : 2U; }
+
+// Elements from the first to the last of `rows` rows of `width`.
+size_t extent(size_t rows, size_t stride, size_t width) { return (rows - 1U) * stride + width; }
+
+// Geometry of the cache; 0 or the refusal.
+int check_cache(const qllm_kv_batch* c, const char* what) {
+  const std::string who(what);
+  if (!c || !c->sequences || !c->kv_heads) return fail(QLLM_INVALID_ARGUMENT, "invalid " + who + " batch");
+  if (c->sequences > 65535U || c->kv_heads > 4096U)
+    return fail(QLLM_INVALID_ARGUMENT, who + " takes at most 65535 sequences and 4096 kv heads");
+  if (c->head_dim != 64U && c->head_dim != 128U && c->head_dim != 192U && c->head_dim != 256U)
+    return fail(QLLM_INVALID_ARGUMENT, who + " needs head_dim 64, 128, 192 or 256");
+  return 0;
+}
+int check_pages(const qllm_kv_batch* c, const char* what) {
+  const std::string who(what);
+  if (!c->page_tables || !aligned(c->page_tables, 8U) || !c->pages_per_sequence || c->encoding > QLLM_KV_Q8)
+    return fail(QLLM_INVALID_ARGUMENT, "invalid " + who + " cache");
+  if (!c->page_tokens || c->page_tokens % 16U || c->layer_offset % 16U)
+    return fail(QLLM_INVALID_ARGUMENT, who + " needs page_tokens and layer_offset in multiples of 16");
+  if (static_cast<uint64_t>(c->pages_per_sequence) * c->page_tokens >= 0x80000000ULL)
+    return fail(QLLM_INVALID_ARGUMENT, who + " takes fewer than 2^31 slots per sequence");
+  return 0;
+}
+
+// Rows that are read or written in 16-byte words.
+bool rows_ok(const void* p, size_t stride, uint32_t type, size_t width) {
+  return p && aligned(p, 16U) && stride >= width && stride * row_bytes(type) % 16U == 0U;
+}
+
+}  // namespace
+
+extern "C" {
+
+int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, const void* qkv, size_t qkv_stride,
+                              uint32_t rows, uint32_t q_heads, uint32_t rotary_dim, const float* q_norm,
+                              const float* k_norm, float eps, const float* inv_freq, const uint32_t* positions,
+                              const uint32_t* row_sequence, const uint32_t* row_slot, void* query, size_t query_stride,
+                              void* key, size_t key_stride, uint32_t* slot_positions, size_t slot_stride,
+                              void* stream) {
+  const char* who = "QK norm / RoPE / KV store";
+  int rc = check_cache(cache, who);
+  if (rc) return rc;
+  if (row_slot && (rc = check_pages(cache, who))) return rc;
+  if (!rows || !q_heads || q_heads > 65536U || row_type > QLLM_ROW_F16 || !q_norm || !k_norm || !positions ||
+      !(eps >= 0.0F) || std::isinf(eps))
+    return fail(QLLM_INVALID_ARGUMENT, "invalid QK norm / RoPE / KV store batch");
+  if (rotary_dim > cache->head_dim || rotary_dim % 16U || (rotary_dim && !inv_freq))
+    return fail(QLLM_INVALID_ARGUMENT, "QK norm / RoPE / KV store needs a rotary_dim that is a multiple of 16 and at most head_dim");
+  if (row_slot && !row_sequence && rows > cache->sequences)
+    return fail(QLLM_INVALID_ARGUMENT, "QK norm / RoPE / KV store: without row_sequence there is at most one row per sequence");
+  const size_t q_width = static_cast<size_t>(q_heads) * cache->head_dim, kv_width = static_cast<size_t>(cache->kv_heads) * cache->head_dim;
+  const size_t e = row_bytes(row_type);
+  if (!rows_ok(qkv, qkv_stride, row_type, q_width + 2U * kv_width) || !rows_ok(query, query_stride, row_type, q_width) ||
+      (key && !rows_ok(key, key_stride, row_type, kv_width)))
+    return fail(QLLM_INVALID_ARGUMENT,
+                "QK norm / RoPE / KV store needs rows on 16-byte boundaries, strides that hold a row and are multiples of 16 bytes");
+  if (slot_positions && (!row_slot || slot_stride < kv_capacity(*cache)))
+    return fail(QLLM_INVALID_ARGUMENT, "QK norm / RoPE / KV store: slot_positions needs row_slot and a stride that holds every slot");
+  // in place is every row's own head over itself; any other sharing would be overwritten before it is read
+  const size_t in = extent(rows, qkv_stride, q_width + 2U * kv_width) * e;
+  const size_t q_out = extent(rows, query_stride, q_width) * e, k_out = key ? extent(rows, key_stride, kv_width) * e : 0U;
+  const uint8_t* base = static_cast<const uint8_t*>(qkv);
+  const bool query_in_place = query == qkv && query_stride == qkv_stride;
+  const bool key_in_place = key == base + q_width * e && key_stride == qkv_stride;
+  const bool both_in_place = query_in_place && key_in_place;
+  if ((!query_in_place && overlap(query, q_out, qkv, in)) || (key && !key_in_place && overlap(key, k_out, qkv, in)) ||
+      (key && !both_in_place && overlap(key, k_out, query, q_out)))
+    return fail(QLLM_INVALID_ARGUMENT, "QK norm / RoPE / KV store: rows overlap and are not in place");
+  NormRopeStoreArgs a{*cache, row_type, qkv, qkv_stride, rows, q_heads, rotary_dim, q_norm, k_norm, eps, inv_freq, positions,
+                      row_sequence, row_slot, query, query_stride, key, key_stride, slot_positions, slot_stride};
+  return launch_norm_rope_store(a, static_cast<cudaStream_t>(stream));
+}
+
+size_t qllm_k_decode_attention_workspace_bytes(const qllm_kv_batch* cache, uint32_t q_heads, int weights) {
+  if (!cache) return 0U;
+  return decode_attention_workspace_bytes(*cache, q_heads, weights != 0);
+}
+
+int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const void* query, size_t query_stride,
+                            const uint32_t* lengths, uint32_t q_heads, float scale, const float* weights_in,
+                            float* weights_out, size_t weights_stride, void* out, size_t out_stride, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  const char* who = "decode attention";
+  int rc = check_cache(cache, who);
+  if (rc || (rc = check_pages(cache, who))) return rc;
+  if (!q_heads || q_heads > 65536U || q_heads % cache->kv_heads || row_type > QLLM_ROW_F16 || !lengths || !workspace ||
+      !std::isfinite(scale))
+    return fail(QLLM_INVALID_ARGUMENT, "invalid decode attention batch");
+  const size_t width = static_cast<size_t>(q_heads) * cache->head_dim, e = row_bytes(row_type);
+  if (!rows_ok(query, query_stride, row_type, width) || !rows_ok(out, out_stride, row_type, width))
+    return fail(QLLM_INVALID_ARGUMENT,
+                "decode attention needs rows on 16-byte boundaries, strides that hold a row and are multiples of 16 bytes");
+  if (overlap(query, extent(cache->sequences, query_stride, width) * e, out, extent(cache->sequences, out_stride, width) * e))
+    return fail(QLLM_INVALID_ARGUMENT, "decode attention: query and out overlap");
+  if (weights_in && !weights_out) return fail(QLLM_INVALID_ARGUMENT, "decode attention: weights_in without weights_out");
+  if (weights_out) {
+    if (weights_stride < kv_capacity(*cache))
+      return fail(QLLM_INVALID_ARGUMENT, "decode attention: the weights' stride does not hold every slot");
+    const size_t bytes = extent(static_cast<size_t>(cache->sequences) * cache->kv_heads, weights_stride, kv_capacity(*cache)) * sizeof(float);
+    if (weights_in && weights_in != weights_out && overlap(weights_in, bytes, weights_out, bytes))
+      return fail(QLLM_INVALID_ARGUMENT, "decode attention: weights overlap and are not in place");
+  }
+  if (!aligned(workspace, 16U) || workspace_bytes < decode_attention_workspace_bytes(*cache, q_heads, weights_out != nullptr))
+    return fail(QLLM_INVALID_ARGUMENT, "decode attention workspace is too small or not on a 16-byte boundary");
+  DecodeAttentionArgs a{*cache, row_type, query, query_stride, lengths, q_heads, scale, weights_in, weights_out, weights_stride,
+                        out, out_stride, workspace};
+  return launch_decode_attention(a, static_cast<cudaStream_t>(stream));
+}
+
+size_t qllm_k_kv_evict_workspace_bytes(const qllm_kv_batch* cache, uint32_t budget) {
+  if (!cache) return 0U;
+  return kv_evict_workspace_bytes(*cache, budget);
+}
+
+int qllm_k_kv_evict(const qllm_kv_batch* cache, const uint32_t* lengths_in, uint32_t* lengths_out,
+                    const uint32_t* next_positions, uint32_t budget, uint32_t recent, uint32_t sinks,
+                    const float* weights_in, float* weights_out, const uint32_t* positions_in, uint32_t* positions_out,
+                    size_t stride, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "KV eviction";
+  int rc = check_cache(cache, who);
+  if (rc || (rc = check_pages(cache, who))) return rc;
+  if (!lengths_in || !lengths_out || !next_positions || !weights_in || !weights_out || !positions_in || !positions_out || !workspace)
+    return fail(QLLM_INVALID_ARGUMENT, "invalid KV eviction batch");
+  if (!budget || static_cast<uint64_t>(recent) + sinks > budget)
+    return fail(QLLM_INVALID_ARGUMENT, "KV eviction needs a budget that holds the recent tokens and the sinks");
+  if (stride < kv_capacity(*cache))
+    return fail(QLLM_INVALID_ARGUMENT, "KV eviction: the stride does not hold every slot");
+  const size_t bytes = extent(static_cast<size_t>(cache->sequences) * cache->kv_heads, stride, kv_capacity(*cache)) * 4U;
+  if ((weights_in != weights_out && overlap(weights_in, bytes, weights_out, bytes)) ||
+      (positions_in != positions_out && overlap(positions_in, bytes, positions_out, bytes)) ||
+      overlap(weights_out, bytes, positions_in, bytes) || overlap(weights_out, bytes, positions_out, bytes) ||
+      overlap(weights_in, bytes, positions_out, bytes))
+    return fail(QLLM_INVALID_ARGUMENT, "KV eviction: arrays overlap and are not in place");
+  const size_t list = cache->sequences * sizeof(uint32_t);
+  if ((lengths_in != lengths_out && overlap(lengths_in, list, lengths_out, list)) || overlap(next_positions, list, lengths_out, list))
+    return fail(QLLM_INVALID_ARGUMENT, "KV eviction: arrays overlap and are not in place");
+  if (!aligned(workspace, 16U) || workspace_bytes < kv_evict_workspace_bytes(*cache, budget))
+    return fail(QLLM_INVALID_ARGUMENT, "KV eviction workspace is too small or not on a 16-byte boundary");
+  KvEvictArgs a{*cache, lengths_in, lengths_out, next_positions, budget, recent, sinks, weights_in, weights_out, positions_in,
+                positions_out, stride, workspace};
+  return launch_kv_evict(a, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

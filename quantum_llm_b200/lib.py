@@ -6,6 +6,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libqllm_b200.so")
 
 KV_F16, KV_Q4H, KV_Q8 = 0, 1, 2
+ROW_F32, ROW_BF16, ROW_F16 = 0, 1, 2
+PADDING_SLOT = 0xFFFFFFFF   # QLLM_PADDING_SLOT
 TP_HANDLE_BYTES = 64   # QLLM_TP_HANDLE_BYTES
 
 
@@ -70,6 +72,12 @@ class Request(C.Structure):
 class ExactResult(C.Structure):
     _fields_ = [("emitted_tokens", C.c_uint32 * 8), ("emitted_count", C.c_uint32),
                 ("next_token", C.c_uint32), ("positions_advanced", C.c_uint32), ("rejected", C.c_uint32)]
+
+
+class KvBatch(C.Structure):
+    _fields_ = [("page_tables", C.c_void_p), ("layer_offset", C.c_size_t)] + \
+               [(n, C.c_uint32) for n in ("sequences", "pages_per_sequence", "page_tokens", "encoding",
+                                          "kv_heads", "head_dim")]
 
 
 u8, u32, u64, f32, f64, vp, sz, ci = (C.c_uint8, C.c_uint32, C.c_uint64, C.c_float, C.c_double,
@@ -141,6 +149,12 @@ SIGNATURES = {
     "qllm_k_kv_layer_bytes": (sz, [u32, u32, u32, u32]),
     "qllm_k_attention_workspace_bytes": (sz, [u32, u32, u32, u32]),
     "qllm_k_attention": (ci, [u32, vp, sz, u32, vp, u32, u32, vp, u32, u32, u32, u32, u32, u32, ci, vp, vp, ci, vp]),
+    "qllm_k_qk_norm_rope_store": (ci, [P(KvBatch), u32, vp, sz, u32, u32, u32, vp, vp, f32, vp, vp, vp, vp, vp, sz, vp, sz,
+                                       vp, sz, vp]),
+    "qllm_k_decode_attention_workspace_bytes": (sz, [P(KvBatch), u32, ci]),
+    "qllm_k_decode_attention": (ci, [P(KvBatch), u32, vp, sz, vp, u32, f32, vp, vp, sz, vp, sz, vp, sz, vp]),
+    "qllm_k_kv_evict_workspace_bytes": (sz, [P(KvBatch), u32]),
+    "qllm_k_kv_evict": (ci, [P(KvBatch), vp, vp, vp, u32, u32, u32, vp, vp, vp, vp, sz, vp, sz, vp]),
     "qllm_k_argmax": (ci, [vp, u32, u32, u32, vp, vp]),
     "qllm_k_topk_workspace_bytes": (sz, [u32, u32, u32]),
     "qllm_k_topk": (ci, [vp, u32, u32, u32, u32, vp, vp, vp, vp]),
