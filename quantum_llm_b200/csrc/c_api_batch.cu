@@ -19,6 +19,9 @@ bool overlap(const void* p, size_t bytes, const void* q, size_t bytes_q) {
 
 size_t row_bytes(uint32_t type) { return type == QLLM_ROW_F32 ? 4U : 2U; }
 
+// Whether `rows` rows `stride` elements apart can be addressed at all.
+bool extent_ok(size_t rows, size_t stride) { return stride <= (static_cast<size_t>(1) << 56U) / rows; }
+
 // Elements from the first to the last of `rows` rows of `width`.
 size_t extent(size_t rows, size_t stride, size_t width) { return (rows - 1U) * stride + width; }
 
@@ -44,8 +47,8 @@ int check_pages(const qllm_kv_batch* c, const char* what) {
 }
 
 // Rows that are read or written in 16-byte words.
-bool rows_ok(const void* p, size_t stride, uint32_t type, size_t width) {
-  return p && aligned(p, 16U) && stride >= width && stride * row_bytes(type) % 16U == 0U;
+bool rows_ok(const void* p, size_t rows, size_t stride, uint32_t type, size_t width) {
+  return p && aligned(p, 16U) && stride >= width && stride * row_bytes(type) % 16U == 0U && extent_ok(rows, stride);
 }
 
 }  // namespace
@@ -71,11 +74,12 @@ int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, con
     return fail(QLLM_INVALID_ARGUMENT, "QK norm / RoPE / KV store: without row_sequence there is at most one row per sequence");
   const size_t q_width = static_cast<size_t>(q_heads) * cache->head_dim, kv_width = static_cast<size_t>(cache->kv_heads) * cache->head_dim;
   const size_t e = row_bytes(row_type);
-  if (!rows_ok(qkv, qkv_stride, row_type, q_width + 2U * kv_width) || !rows_ok(query, query_stride, row_type, q_width) ||
-      (key && !rows_ok(key, key_stride, row_type, kv_width)))
+  if (!rows_ok(qkv, rows, qkv_stride, row_type, q_width + 2U * kv_width) || !rows_ok(query, rows, query_stride, row_type, q_width) ||
+      (key && !rows_ok(key, rows, key_stride, row_type, kv_width)))
     return fail(QLLM_INVALID_ARGUMENT,
                 "QK norm / RoPE / KV store needs rows on 16-byte boundaries, strides that hold a row and are multiples of 16 bytes");
-  if (slot_positions && (!row_slot || slot_stride < kv_capacity(*cache)))
+  if (slot_positions && (!row_slot || slot_stride < kv_capacity(*cache) ||
+                         !extent_ok(static_cast<size_t>(cache->sequences) * cache->kv_heads, slot_stride)))
     return fail(QLLM_INVALID_ARGUMENT, "QK norm / RoPE / KV store: slot_positions needs row_slot and a stride that holds every slot");
   // in place is every row's own head over itself; any other sharing would be overwritten before it is read
   const size_t in = extent(rows, qkv_stride, q_width + 2U * kv_width) * e;
@@ -107,15 +111,17 @@ int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const
   if (!q_heads || q_heads > 65536U || q_heads % cache->kv_heads || row_type > QLLM_ROW_F16 || !lengths || !workspace ||
       !std::isfinite(scale))
     return fail(QLLM_INVALID_ARGUMENT, "invalid decode attention batch");
+  if (static_cast<uint64_t>(cache->sequences) * q_heads > (1U << 28U))
+    return fail(QLLM_INVALID_ARGUMENT, "decode attention takes at most 2^28 query heads over all sequences");
   const size_t width = static_cast<size_t>(q_heads) * cache->head_dim, e = row_bytes(row_type);
-  if (!rows_ok(query, query_stride, row_type, width) || !rows_ok(out, out_stride, row_type, width))
+  if (!rows_ok(query, cache->sequences, query_stride, row_type, width) || !rows_ok(out, cache->sequences, out_stride, row_type, width))
     return fail(QLLM_INVALID_ARGUMENT,
                 "decode attention needs rows on 16-byte boundaries, strides that hold a row and are multiples of 16 bytes");
   if (overlap(query, extent(cache->sequences, query_stride, width) * e, out, extent(cache->sequences, out_stride, width) * e))
     return fail(QLLM_INVALID_ARGUMENT, "decode attention: query and out overlap");
   if (weights_in && !weights_out) return fail(QLLM_INVALID_ARGUMENT, "decode attention: weights_in without weights_out");
   if (weights_out) {
-    if (weights_stride < kv_capacity(*cache))
+    if (weights_stride < kv_capacity(*cache) || !extent_ok(static_cast<size_t>(cache->sequences) * cache->kv_heads, weights_stride))
       return fail(QLLM_INVALID_ARGUMENT, "decode attention: the weights' stride does not hold every slot");
     const size_t bytes = extent(static_cast<size_t>(cache->sequences) * cache->kv_heads, weights_stride, kv_capacity(*cache)) * sizeof(float);
     if (weights_in && weights_in != weights_out && overlap(weights_in, bytes, weights_out, bytes))
@@ -144,7 +150,7 @@ int qllm_k_kv_evict(const qllm_kv_batch* cache, const uint32_t* lengths_in, uint
     return fail(QLLM_INVALID_ARGUMENT, "invalid KV eviction batch");
   if (!budget || static_cast<uint64_t>(recent) + sinks > budget)
     return fail(QLLM_INVALID_ARGUMENT, "KV eviction needs a budget that holds the recent tokens and the sinks");
-  if (stride < kv_capacity(*cache))
+  if (stride < kv_capacity(*cache) || !extent_ok(static_cast<size_t>(cache->sequences) * cache->kv_heads, stride))
     return fail(QLLM_INVALID_ARGUMENT, "KV eviction: the stride does not hold every slot");
   const size_t bytes = extent(static_cast<size_t>(cache->sequences) * cache->kv_heads, stride, kv_capacity(*cache)) * 4U;
   if ((weights_in != weights_out && overlap(weights_in, bytes, weights_out, bytes)) ||

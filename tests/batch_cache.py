@@ -177,7 +177,7 @@ def exact_norm_rope(x, q_heads, kv, hd, rot, q_norm, k_norm, inv, positions, eps
 
 
 def exact_attention(cache, s, n, q, q_heads, scale):
-    """Of one sequence: (out [q_heads, hd], p [q_heads, n], sum p|V|, largest sum |q||K| scale)."""
+    """Of one sequence: (out [q_heads, hd], p [q_heads, n], sum p|V|, largest sum |q||K| scale, sum |V|)."""
     hd, group = cache.hd, q_heads // cache.kv
     k, v, there = cache.values(s, n)
     q = q.double().view(cache.kv, group, hd)
@@ -192,7 +192,8 @@ def exact_attention(cache, s, n, q, q_heads, scale):
     v = torch.where(there[:, None, None], v, torch.zeros_like(v))   # what an absent or masked slot holds does not count
     out = torch.einsum("hgt,thd->hgd", p, v)
     spread = torch.einsum("hgt,thd->hgd", p, v.abs())
-    return out.reshape(q_heads, hd), p.reshape(q_heads, n), spread.reshape(q_heads, hd), size.reshape(q_heads)
+    return out.reshape(q_heads, hd), p.reshape(q_heads, n), spread.reshape(q_heads, hd), size.reshape(q_heads), \
+        v.abs().sum(0).repeat_interleave(group, 0)
 
 
 def exact_evict(w, p, n, following, budget, recent, sinks):

@@ -168,18 +168,18 @@ def test_norm_rope_store_many_rows_and_infinities():
 
 # ------------------------------------------------------------------------------- attention
 
-def attention_bounds(dtype, n, hd, p, spread, size, want):
+def attention_bounds(dtype, n, hd, p, spread, size, want, v_sum):
     """z = scale * q.K is off by d = size * (hd + 8) e: hd additions of products (exact or rounded once), the query
     held in at least 22 bits.  exp2 and its argument's rounding add 8 e (1 + |z|), |z| <= size.  A weight of p is off by
     twice that (itself and the sum it is divided by), and the sums over n keys by 8 sqrt(n) e (a random walk of n
-    roundings, taken eight times).  With 16-bit rows each weight may be rounded to F16 before it meets V: 2^-11, and below 2^-14 of the
-    largest by 2^-25 of it, n times."""
+    roundings, taken eight times).  Before it meets V a weight becomes one F16 term with 16-bit rows (half a step: 2^-11) and
+    two with FP32 rows (2^-22).  F16's smallest step is 2^-24, and the weights are scaled so that the largest (times V's scale) is at
+    least 2^7: whatever its size, a weight is off by up to 2^-25 / 2^7 = 2^-32 of the largest, which meets sum |V|; a quantised V's
+    scales, which the largest includes, differ by less than 2^4 here."""
     rel = 2 * (size * (hd + 8) + 8 * (1 + size)) * E + 8 * math.sqrt(n + 1) * E
-    weight = rel if dtype == F32 else rel + 2.0 ** -11
+    weight = rel + (2.0 ** -22 if dtype == F32 else 2.0 ** -11)
     largest = p.amax(-1) if n else torch.zeros_like(size)
-    v_max = (spread / p.sum(-1, keepdim=True).clamp_min(1e-30)).amax(-1)
-    tiny = 0.0 if dtype == F32 else n * 2.0 ** -25 * largest * v_max
-    out = HALF_STEP[dtype] * want.abs() + weight[:, None] * spread * 1.01 + torch.as_tensor(tiny, device="cuda").reshape(-1, 1)
+    out = HALF_STEP[dtype] * want.abs() + weight[:, None] * spread * 1.01 + 2.0 ** -28 * largest[:, None] * v_sum
     return out + (2.0 ** -25 if dtype == HF16 else 1e-37), rel
 
 
@@ -187,9 +187,9 @@ def check_attention(cache, query, lengths, q_heads, scale, out, weights_in, weig
     group = q_heads // cache.kv
     for s, n in enumerate(lengths):
         n = min(n, cache.capacity)
-        want, p, spread, size = bc.exact_attention(cache, s, n, query[s], q_heads, scale)
+        want, p, spread, size, v_sum = bc.exact_attention(cache, s, n, query[s], q_heads, scale)
         got = out[s].view(q_heads, cache.hd).double()
-        bound, rel = attention_bounds(dtype, n, cache.hd, p, spread, size, want)
+        bound, rel = attention_bounds(dtype, n, cache.hd, p, spread, size, want, v_sum)
         assert bool(got.isfinite().all()), f"sequence {s} of {n}"
         worst = ((got - want).abs() / bound).max()
         assert float(worst) <= 1.0, f"sequence {s} of {n}: {float(worst)} of the bound"
