@@ -3,6 +3,7 @@
 #include <cmath>
 #include <string>
 
+#include "kernels.h"
 #include "kv_batch.cuh"
 
 using namespace qllm;
@@ -43,6 +44,8 @@ int check_pages(const qllm_kv_batch* c, const char* what) {
     return fail(QLLM_INVALID_ARGUMENT, who + " needs page_tokens and layer_offset in multiples of 16");
   if (static_cast<uint64_t>(c->pages_per_sequence) * c->page_tokens >= 0x80000000ULL)
     return fail(QLLM_INVALID_ARGUMENT, who + " takes fewer than 2^31 slots per sequence");
+  if (kv_layer_bytes(c->encoding, 1U, c->kv_heads, c->head_dim) * c->page_tokens >= 0x100000000ULL)
+    return fail(QLLM_INVALID_ARGUMENT, who + " takes pages that hold less than 4 GiB of a layer");
   return 0;
 }
 

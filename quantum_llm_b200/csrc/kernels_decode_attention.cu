@@ -31,6 +31,7 @@
 // equal to that of an F16 row before averaging.  The softmax reference is only moved when p would exceed 2^15 (one
 // vote per tile instead of a reduction) and is set so that the largest p is 2^7 then: F16 holds p down to 2^-32 of
 // the largest, and a quantised V's scale is counted into the reference so that this holds for p times scale.
+#include "kernels.h"
 #include "kv_batch.cuh"
 #include "launch.cuh"
 
@@ -41,9 +42,10 @@ namespace {
 constexpr uint32_t kWarps = 4;
 constexpr uint32_t kThreads = 32 * kWarps;
 constexpr uint32_t kUnit = 64;          // tokens
+constexpr uint32_t kItemBytes = 96U * 1024U;  // what a block could read in the time an item costs it beside its tokens
 constexpr uint32_t kMaxBlocks = 512;    // of the first launch; places in the workspace
 constexpr uint32_t kHeads = 8;          // query heads of an item per kv head
-constexpr uint32_t kJoinThreads = 256;
+constexpr uint32_t kWeightTokens = 4 * kThreads;
 // log2: the largest p of a warp stands between 2^kLift (when the reference was set) and 2^kTop < 65504
 constexpr float kLift = 7.0F, kTop = 15.0F;
 constexpr float kLog2e = 1.4426950408889634F;
@@ -59,7 +61,9 @@ struct Plan {
   uint32_t heads;          // kv heads of an item
   uint32_t group, tiles;   // query heads per kv head, and tiles of eight of them
   uint32_t items;          // per sequence
-  size_t place;            // floats of one place: heads * 8 * (2 + head_dim)
+  uint32_t cost;           // of an item beside its tokens, in units
+  uint32_t rows;           // of one place: heads * 8
+  size_t place;            // floats of one place: [rows] maxima, [rows] sums, [rows][head_dim] outputs
   float* partials;         // [kMaxBlocks][2][place]
   uint2* spans;            // [sequences * items]: first and last block of an item
   float* lse;              // [sequences, q_heads], log2 (weights only)
@@ -73,7 +77,10 @@ Plan plan_of(const KvBatch& c, uint32_t q_heads, bool weights, void* workspace) 
   p.group = q_heads / c.kv_heads;
   p.tiles = (p.group + kHeads - 1U) / kHeads;
   p.items = c.kv_heads / p.heads * p.tiles;
-  p.place = static_cast<size_t>(p.heads) * kHeads * (2U + c.head_dim);
+  const size_t unit = kUnit * p.heads * kv_layer_bytes(c.encoding, 1U, 1U, c.head_dim);
+  p.cost = static_cast<uint32_t>((kItemBytes + unit - 1U) / unit);
+  p.rows = p.heads * kHeads;
+  p.place = static_cast<size_t>(p.rows) * (2U + c.head_dim);
   uint8_t* at = static_cast<uint8_t*>(workspace);
   size_t n = 0;
   const auto take = [&](size_t bytes) {
@@ -158,8 +165,9 @@ __device__ __forceinline__ uint32_t bytes_to_half(uint32_t v) {
 template <int ENC, int HD>
 struct Layout {
   static constexpr bool kStaged = ENC == QLLM_KV_Q8;
-  // blocks of 16 keys that a warp takes at a time: 32 registers of K and of V (HD 64, 128, 256), 24 - 48 (192)
-  static constexpr int kBlocks = ENC == QLLM_KV_F16 ? (HD == 64 ? 2 : 1) : ENC == QLLM_KV_Q4H ? (HD <= 128 ? 4 : 2) : 1;
+  // blocks of 16 keys that a warp takes at a time: 16 - 64 registers of K and of V (Q4H, HD 128: 4 blocks spill, 31 us
+  // against 25 us with 2 for one sequence of 32768)
+  static constexpr int kBlocks = ENC == QLLM_KV_F16 ? (HD == 64 ? 2 : 1) : ENC == QLLM_KV_Q4H ? (HD == 64 ? 4 : 2) : 1;
   static constexpr int kRegs = ENC == QLLM_KV_F16 ? HD / 4 : ENC == QLLM_KV_Q4H ? HD / 16 : 1;  // of K, and of V, per block
   static constexpr int kKWords = ENC == QLLM_KV_Q4H ? (HD % 128 == 0 ? 4 : 2) : 4;      // words per load
   static constexpr int kVWords = ENC == QLLM_KV_Q4H ? (HD == 128 ? 2 : HD == 256 ? 4 : 1) : 4;
@@ -187,9 +195,30 @@ struct Layout {
 
 // Where the keys of a 16-key block lie.
 struct Block {
-  const uint8_t* layer;  // null: no page
+  const uint8_t* keys;   // K codes (values) of its first token and the warp's kv head; null: no page
   uint32_t place;        // of its first token in the page
   uint32_t count;        // keys that count, 0..16
+};
+
+// Walks every `step` tokens from `first` through the pages of a sequence, without a division after the start.
+struct Cursor {
+  uint32_t token, page, place;
+  uint32_t step, step_pages, step_place;
+  __device__ __forceinline__ Cursor(const KvBatch& c, uint32_t first, uint32_t step_) : token(first), step(step_) {
+    page = first / c.page_tokens;
+    place = first - page * c.page_tokens;
+    step_pages = step / c.page_tokens;
+    step_place = step - step_pages * c.page_tokens;
+  }
+  __device__ __forceinline__ void advance(const KvBatch& c) {
+    token += step;
+    page += step_pages;
+    place += step_place;
+    if (place >= c.page_tokens) {
+      place -= c.page_tokens;
+      ++page;
+    }
+  }
 };
 
 template <typename T, int ENC, int HD>
@@ -199,11 +228,14 @@ struct Traits {
   static constexpr int kSteps = HD / 16;
   static constexpr bool kQueryInRegisters = HD <= 128;
   static constexpr int kBlocksPerSm = HD <= 128 ? 3 : 2;
-  static constexpr size_t kFragmentBytes = static_cast<size_t>(kSteps) * 32 * kTerms * sizeof(uint2);  // of one kv head
+  // the queries of one kv head: rows 16 bytes apart from a multiple of 128 (free of bank conflicts), then fragments in their place
+  static constexpr int kQueryPitch = HD * static_cast<int>(sizeof(T)) + 16;
+  static constexpr size_t kQueryBytes = static_cast<size_t>(kHeads) * kQueryPitch;
+  static_assert(kQueryBytes >= static_cast<size_t>(kSteps) * 32 * kTerms * sizeof(uint2), "fragments fit");
   static constexpr int kRow = HD + 4;  // floats of one head in the merge area
   static constexpr size_t kMergeBytes = (kWarps * kHeads * kRow + 2 * kWarps * kHeads) * sizeof(float);
   static constexpr size_t kRingBytes = Layout<ENC, HD>::kStaged ? static_cast<size_t>(kWarps) * Layout<ENC, HD>::kStages * Layout<ENC, HD>::kStage : 0;
-  static constexpr size_t kShared = (kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes) + kFragmentBytes * (ENC == QLLM_KV_Q8 ? 4 : 1);
+  static constexpr size_t kShared = (kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes) + kQueryBytes * (ENC == QLLM_KV_Q8 ? 4 : 1);
 };
 
 // State of the online softmax and of the output in one warp: heads 2 c and 2 c + 1 of the lane.
@@ -279,22 +311,9 @@ __device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from, bool th
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 
-// Block `index` of the warp's blocks in tokens [first, last) of a sequence.
-__device__ __forceinline__ Block find_block(const KvBatch& c, uint32_t sequence, uint32_t first, uint32_t last, uint32_t index,
-                                            uint32_t phase, uint32_t phases) {
-  const uint64_t t = first + 16ULL * (phase + static_cast<uint64_t>(phases) * index);
-  Block b{nullptr, 0U, 0U};
-  if (t < last) {
-    const uint32_t page = static_cast<uint32_t>(t) / c.page_tokens;
-    b.place = static_cast<uint32_t>(t) - page * c.page_tokens;
-    b.layer = kv_page(c, sequence, page);
-    b.count = b.layer ? min(16U, last - static_cast<uint32_t>(t)) : 0U;
-  }
-  return b;
-}
 __device__ __forceinline__ Block take_block(const Block& mine, int lane) {
   Block b;
-  b.layer = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffU, reinterpret_cast<unsigned long long>(mine.layer), lane));
+  b.keys = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffU, reinterpret_cast<unsigned long long>(mine.keys), lane));
   b.place = __shfl_sync(0xffffffffU, mine.place, lane);
   b.count = __shfl_sync(0xffffffffU, mine.count, lane);
   return b;
@@ -317,6 +336,35 @@ struct Warp {
     return fragments[(step * X::kTerms + term) * 32 + lane];
   }
 
+  // Offsets inside a page's layer are below 2^32 (checked by the host).
+  uint32_t stride;       // bytes from a token's record to the next token's (of one head)
+  uint32_t to_values;    // from K records to V records
+  uint32_t records;      // of K in a page
+  __device__ __forceinline__ void layout() {
+    records = a.cache.page_tokens * a.cache.kv_heads;
+    stride = ENC == QLLM_KV_F16 ? a.cache.kv_heads * HD * 2U : ENC == QLLM_KV_Q8 ? a.cache.kv_heads * (HD + 2U) : HD / 2U;
+    to_values = records * (ENC == QLLM_KV_F16 ? HD * 2U : ENC == QLLM_KV_Q8 ? HD + 2U : HD / 2U + 2U);
+  }
+  __device__ __forceinline__ Block block_at(const Cursor& at, uint32_t last) const {
+    Block b{nullptr, at.place, 0U};
+    if (at.token < last) {
+      const uint8_t* layer = kv_page(a.cache, sequence, at.page);
+      if (layer) {
+        const uint32_t offset = ENC == QLLM_KV_F16   ? at.place * stride + kv_head * (HD * 2U)
+                                : ENC == QLLM_KV_Q8 ? at.place * stride + kv_head * (HD + 2U)
+                                                     : (kv_head * a.cache.page_tokens + at.place) * stride;
+        b.keys = layer + offset;
+        b.count = min(16U, last - at.token);
+      }
+    }
+    return b;
+  }
+  // Q4H: the scales of a block's keys
+  __device__ __forceinline__ const uint8_t* scales_of(const Block& b) const {
+    const uint32_t record = kv_head * a.cache.page_tokens + b.place;
+    return b.keys + (records * (HD / 2U) - record * (HD / 2U) + record * 2U);
+  }
+
   // ---- registers (F16, Q4H)
   __device__ __forceinline__ void load_keys(const Block& b, uint32_t (&k)[L::kRegs], uint32_t& scales) {
     if (b.count == 0U) {
@@ -325,56 +373,38 @@ struct Warp {
       scales = 0U;
       return;
     }
+    const uint8_t* p = b.keys + 2U * r * stride + (ENC == QLLM_KV_F16 ? 16U : 4U * L::kKWords) * c;
     if constexpr (ENC == QLLM_KV_F16) {
-      const size_t stride = static_cast<size_t>(a.cache.kv_heads) * HD * 2U;
-      const uint8_t* p = b.layer + (b.place + 2U * r) * stride + static_cast<size_t>(kv_head) * HD * 2U + 16U * c;
 #pragma unroll
       for (int row = 0; row < 2; ++row)
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) load_words<4>(&k[row * (HD / 8) + 4 * j], p + row * stride + 64 * j);
     } else {
-      const size_t record = static_cast<size_t>(kv_head) * a.cache.page_tokens + b.place + 2U * r;
-      const uint8_t* p = b.layer + record * (HD / 2) + 4 * L::kKWords * c;
 #pragma unroll
       for (int row = 0; row < 2; ++row)
 #pragma unroll
         for (int j = 0; j < HD / 32 / L::kKWords; ++j)
           load_words<L::kKWords>(&k[row * (HD / 32) + L::kKWords * j], p + row * (HD / 2) + 16 * L::kKWords * j);
-      load_words<1>(&scales, b.layer + static_cast<size_t>(a.cache.page_tokens) * a.cache.kv_heads * (HD / 2) + record * 2U);
+      load_words<1>(&scales, scales_of(b) + 4U * r);
     }
   }
   __device__ __forceinline__ void load_values(const Block& b, uint32_t (&v)[L::kRegs], uint32_t& scales) {
-    const size_t records = static_cast<size_t>(a.cache.page_tokens) * a.cache.kv_heads;
+    const uint8_t* p = b.keys + to_values + 4U * c * stride + (ENC == QLLM_KV_F16 ? 16U : 4U * L::kVWords) * r;
+    constexpr int kWordsOnce = L::kVWords, kLoads = HD * (ENC == QLLM_KV_F16 ? 4 : 1) / 64 / kWordsOnce;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const bool there = 4U * c + q < b.count;
-      if constexpr (ENC == QLLM_KV_F16) {
-        const size_t stride = static_cast<size_t>(a.cache.kv_heads) * HD * 2U;
-        const uint8_t* p = b.layer + records * HD * 2U + (b.place + 4U * c + q) * stride + static_cast<size_t>(kv_head) * HD * 2U + 16U * r;
 #pragma unroll
-        for (int j = 0; j < HD / 64; ++j) {
-          uint32_t* d = &v[(q * (HD / 64) + j) * 4];
-          d[0] = d[1] = d[2] = d[3] = 0U;
-          if (there) load_words<4>(d, p + 128 * j);
-        }
-      } else {
-        const size_t record = static_cast<size_t>(kv_head) * a.cache.page_tokens + b.place + 4U * c + q;
-        const uint8_t* p = b.layer + records * (HD / 2 + 2) + record * (HD / 2) + 4 * L::kVWords * r;
+      for (int j = 0; j < kLoads; ++j) {
+        uint32_t* d = &v[(q * kLoads + j) * kWordsOnce];
 #pragma unroll
-        for (int j = 0; j < HD / 64 / L::kVWords; ++j) {
-          uint32_t* d = &v[q * (HD / 64) + L::kVWords * j];
-#pragma unroll
-          for (int i = 0; i < L::kVWords; ++i) d[i] = 0U;
-          if (there) load_words<L::kVWords>(d, p + 32 * L::kVWords * j);
-        }
+        for (int i = 0; i < kWordsOnce; ++i) d[i] = 0U;
+        if (there) load_words<kWordsOnce>(d, p + q * stride + 32 * kWordsOnce * j);
       }
     }
     scales = 0U;
     if constexpr (ENC == QLLM_KV_Q4H) {
-      if (b.count) {
-        const size_t record = static_cast<size_t>(kv_head) * a.cache.page_tokens + b.place + 2U * r;
-        load_words<1>(&scales, b.layer + records * (HD / 2 + 2) + records * (HD / 2) + record * 2U);
-      }
+      if (b.count) load_words<1>(&scales, scales_of(b) + to_values + 4U * r);
     }
   }
   template <int kQ>
@@ -439,110 +469,118 @@ struct Warp {
 
   // ---- through shared memory (Q8): rows of windows, key 2r in row r, key 2r + 1 in row r + 8
   __device__ __forceinline__ void stage(const Block& b, uint32_t to) {
-    const size_t stride = static_cast<size_t>(a.cache.kv_heads) * (HD + 2);
-    const size_t records = static_cast<size_t>(a.cache.page_tokens) * a.cache.kv_heads;
-    const uint8_t* base = b.layer + b.place * stride + static_cast<size_t>(kv_head) * (HD + 2);
+    constexpr int kCopies = (16 * L::kWindows + 31) / 32;  // of a lane, for K and for V
+    const uint8_t* base = b.keys ? b.keys : reinterpret_cast<const uint8_t*>(a.cache.page_tables);
 #pragma unroll
-    for (int value = 0; value < 2; ++value)
-      for (uint32_t i = lane; i < 16U * L::kWindows; i += 32U) {
-        const uint32_t key = i / L::kWindows, window = i % L::kWindows;
-        const uintptr_t record = reinterpret_cast<uintptr_t>(base + value * records * (HD + 2) + key * stride);
-        const uint32_t row = value * 16U + key / 2U + 8U * (key & 1U);
-        const bool there = key < b.count;
-        copy16(to + row * L::kPitch + 16U * window,
-               there ? reinterpret_cast<const uint8_t*>(record & ~static_cast<uintptr_t>(15U)) + 16U * window
-                     : reinterpret_cast<const uint8_t*>(a.cache.page_tables), there);
-      }
+    for (int i = 0; i < kCopies; ++i) {
+      const uint32_t index = lane + 32U * i, key = index / L::kWindows, window = index % L::kWindows;
+      if (index >= 16U * L::kWindows) break;
+      const uintptr_t record = reinterpret_cast<uintptr_t>(base) + (b.keys ? key * stride : 0U);
+      const uint8_t* from = reinterpret_cast<const uint8_t*>(record & ~static_cast<uintptr_t>(15U)) + 16U * window;
+      const uint32_t row = key / 2U + 8U * (key & 1U);
+      copy16(to + row * L::kPitch + 16U * window, from, key < b.count);
+      copy16(to + (16U + row) * L::kPitch + 16U * window, from + (b.keys ? to_values : 0U), key < b.count);  // V begins on 16 bytes
+    }
   }
-  // where a record begins in its row
-  __device__ __forceinline__ uint32_t shift_of(const Block& b, uint32_t key, bool value) const {
-    const size_t stride = static_cast<size_t>(a.cache.kv_heads) * (HD + 2);
-    const size_t records = static_cast<size_t>(a.cache.page_tokens) * a.cache.kv_heads;
-    return static_cast<uint32_t>((b.place + key) * stride + static_cast<size_t>(kv_head) * (HD + 2) +
-                                 (value ? records * (HD + 2) : 0U)) & 15U;  // pages and layers begin on 16 bytes
+  // where a record begins in its row (K and V alike; pages and layers begin on 16 bytes)
+  __device__ __forceinline__ uint32_t shift_of(const Block& b, uint32_t key) const {
+    return (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(b.keys)) + key * stride) & 15U;
   }
 
-  // Tokens [first, last) of the sequence, every `phases`-th block of 16 from `phase` on.
-  template <int kQ>
-  __device__ __forceinline__ void tokens(const uint2 (&q)[kQ], uint32_t first, uint32_t last, uint32_t phase, uint32_t phases,
-                                         float* scores, size_t capacity, uint32_t heads_here, uint8_t* ring) {
+  // The warp's part of tokens [first, last) of the sequence: every `phases`-th block of 16 from `phase` on.  begin() starts
+  // the first loads, which need no query; tokens() does the rest.
+  struct Start {
+    uint32_t k[L::kStaged ? 1 : kN][L::kRegs], v[L::kStaged ? 1 : kN][L::kRegs], kscale[L::kStaged ? 1 : kN], vscale[L::kStaged ? 1 : kN];
+    Block now[L::kStaged ? L::kStages : kN];
+    Block ahead;
+    uint32_t tiles;
+  };
+  __device__ __forceinline__ void begin(Start& x, Cursor& at, uint32_t first, uint32_t last, uint32_t phase, uint32_t phases, uint32_t ring) {
     const uint32_t blocks = (last - first + 15U) / 16U;
     const uint32_t mine = blocks > phase ? (blocks - phase + phases - 1U) / phases : 0U;
-    const uint32_t tiles = (mine + kN - 1U) / kN;
+    x.tiles = (mine + kN - 1U) / kN;
     if constexpr (!L::kStaged) {
-      uint32_t k[kN][L::kRegs], v[kN][L::kRegs], kscale[kN], vscale[kN];
-      Block now[kN];
-      Block ahead = find_block(a.cache, sequence, first, last, lane % kN, phase, phases);
+      const Block b0 = block_at(at, last);
+      at.advance(a.cache);
 #pragma unroll
       for (int b = 0; b < kN; ++b) {
-        now[b] = take_block(ahead, b);
-        load_keys(now[b], k[b], kscale[b]);
+        x.now[b] = take_block(b0, b);
+        load_keys(x.now[b], x.k[b], x.kscale[b]);
       }
 #pragma unroll
-      for (int b = 0; b < kN; ++b) load_values(now[b], v[b], vscale[b]);
-      ahead = find_block(a.cache, sequence, first, last, kN + lane % kN, phase, phases);
-      for (uint32_t tile = 0; tile < tiles; ++tile) {
+      for (int b = 0; b < kN; ++b) load_values(x.now[b], x.v[b], x.vscale[b]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < L::kStages - 1; ++i) {
+        x.now[i] = block_at(at, last);
+        at.advance(a.cache);
+        if (static_cast<uint32_t>(i) < x.tiles) stage(x.now[i], ring + i * L::kStage);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+    }
+    x.ahead = block_at(at, last);
+    at.advance(a.cache);
+  }
+  template <int kQ>
+  __device__ __forceinline__ void tokens(Start& x, Cursor& at, const uint2 (&q)[kQ], uint32_t first, uint32_t last, uint32_t phase, uint32_t phases,
+                                         float* scores, size_t capacity, uint32_t heads_here, uint8_t* ring) {
+    if constexpr (!L::kStaged) {
+      for (uint32_t tile = 0; tile < x.tiles; ++tile) {
         float s[kN][4], vs[kN][2];
         uint32_t count[kN];
 #pragma unroll
         for (int b = 0; b < kN; ++b) {
-          score(q, k[b], s[b]);
-          count[b] = now[b].count;
-          const float2 ks = ENC == QLLM_KV_Q4H ? unpack_half(kscale[b]) : make_float2(1.0F, 1.0F);
+          score(q, x.k[b], s[b]);
+          count[b] = x.now[b].count;
+          const float2 ks = ENC == QLLM_KV_Q4H ? unpack_half(x.kscale[b]) : make_float2(1.0F, 1.0F);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             s[b][h] = 2U * r < count[b] ? s[b][h] * (ks.x * scale[h]) : -INFINITY;
             s[b][2 + h] = 2U * r + 1U < count[b] ? s[b][2 + h] * (ks.y * scale[h]) : -INFINITY;
           }
-          put_scores(scores, capacity, heads_here, first + 16U * (phase + phases * (tile * kN + b)), last, s[b]);
+          if (scores) put_scores(scores, capacity, heads_here, first + 16U * (phase + phases * (tile * kN + b)), last, s[b]);
         }
-        const bool more = tile + 1U < tiles;
+        const bool more = tile + 1U < x.tiles;
         if (more) {
 #pragma unroll
           for (int b = 0; b < kN; ++b) {
-            now[b] = take_block(ahead, b);
-            load_keys(now[b], k[b], kscale[b]);
+            x.now[b] = take_block(x.ahead, b);
+            load_keys(x.now[b], x.k[b], x.kscale[b]);
           }
         }
 #pragma unroll
         for (int b = 0; b < kN; ++b) {
-          const float2 f = ENC == QLLM_KV_Q4H ? unpack_half(vscale[b]) : make_float2(1.0F, 1.0F);
+          const float2 f = ENC == QLLM_KV_Q4H ? unpack_half(x.vscale[b]) : make_float2(1.0F, 1.0F);
           vs[b][0] = 2U * r < count[b] ? f.x : 0.0F;
           vs[b][1] = 2U * r + 1U < count[b] ? f.y : 0.0F;
         }
         softmax_tile<HD, kN, ENC != QLLM_KV_F16>(run, s, vs);
 #pragma unroll
-        for (int b = 0; b < kN; ++b) add_values(v[b], s[b]);
+        for (int b = 0; b < kN; ++b) add_values(x.v[b], s[b]);
         if (more) {
 #pragma unroll
-          for (int b = 0; b < kN; ++b) load_values(now[b], v[b], vscale[b]);
-          ahead = find_block(a.cache, sequence, first, last, (tile + 2U) * kN + lane % kN, phase, phases);
+          for (int b = 0; b < kN; ++b) load_values(x.now[b], x.v[b], x.vscale[b]);
+          x.ahead = block_at(at, last);
+          at.advance(a.cache);
         }
       }
     } else {
       const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-      Block held[L::kStages];
-#pragma unroll
-      for (int i = 0; i < L::kStages - 1; ++i) {
-        held[i] = find_block(a.cache, sequence, first, last, i, phase, phases);
-        if (static_cast<uint32_t>(i) < tiles) stage(held[i], base + i * L::kStage);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      }
-      Block ahead = find_block(a.cache, sequence, first, last, L::kStages - 1, phase, phases);
-      for (uint32_t tile0 = 0; tile0 < tiles; tile0 += L::kStages) {
+      for (uint32_t tile0 = 0; tile0 < x.tiles; tile0 += L::kStages) {
 #pragma unroll
         for (int i = 0; i < L::kStages; ++i) {
           const uint32_t tile = tile0 + i;
-          if (tile >= tiles) break;
+          if (tile >= x.tiles) break;
           asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
           __syncwarp();
-          staged_block(q, held[i], ring + i * L::kStage, first + 16U * (phase + phases * tile), last, scores, capacity, heads_here);
+          staged_block(q, x.now[i], ring + i * L::kStage, first + 16U * (phase + phases * tile), last, scores, capacity, heads_here);
           __syncwarp();
           constexpr int kBehind = L::kStages - 1;
-          held[(i + kBehind) % L::kStages] = ahead;
-          if (tile + kBehind < tiles) stage(ahead, base + (i + kBehind) % L::kStages * L::kStage);
+          x.now[(i + kBehind) % L::kStages] = x.ahead;
+          if (tile + kBehind < x.tiles) stage(x.ahead, base + (i + kBehind) % L::kStages * L::kStage);
           asm volatile("cp.async.commit_group;" ::: "memory");
-          ahead = find_block(a.cache, sequence, first, last, tile + kBehind + 1U, phase, phases);
+          x.ahead = block_at(at, last);
+          at.advance(a.cache);
         }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -550,7 +588,6 @@ struct Warp {
   }
   __device__ __forceinline__ void put_scores(float* scores, size_t capacity, uint32_t heads_here, uint64_t token, uint32_t last,
                                              const float (&s)[4]) const {
-    if (!scores) return;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (2U * c + h >= heads_here) continue;
@@ -566,9 +603,9 @@ struct Warp {
     const uint8_t* rows[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      rows[k] = at + (r + 8U * k) * L::kPitch + shift_of(b, 2U * r + k, false);
+      rows[k] = at + (r + 8U * k) * L::kPitch + shift_of(b, 2U * r + k);
       ks[k] = __half2float(*reinterpret_cast<const __half*>(rows[k] + HD));
-      const uint8_t* value = at + (16U + r + 8U * k) * L::kPitch + shift_of(b, 2U * r + k, true);
+      const uint8_t* value = at + (16U + r + 8U * k) * L::kPitch + shift_of(b, 2U * r + k);
       vs[0][k] = 2U * r + k < b.count ? __half2float(*reinterpret_cast<const __half*>(value + HD)) : 0.0F;
     }
 #pragma unroll
@@ -591,14 +628,14 @@ struct Warp {
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int h = 0; h < 2; ++h) s[0][2 * k + h] = 2U * r + k < b.count ? s[0][2 * k + h] * (ks[k] * scale[h]) : -INFINITY;
-    put_scores(scores, capacity, heads_here, token, last, s[0]);
+    if (scores) put_scores(scores, capacity, heads_here, token, last, s[0]);
     softmax_tile<HD, 1, true>(run, s, vs);
     uint32_t hi[2], lo[2] = {0U, 0U};
     weight_fragments<X::kPrecise>(s[0], hi, lo);
     const uint8_t* v[4];
 #pragma unroll
     for (uint32_t k = 0; k < 4U; ++k)
-      v[k] = at + (16U + 2U * c + k / 2U + 8U * (k & 1U)) * L::kPitch + shift_of(b, 4U * c + k, true) + 2U * r;
+      v[k] = at + (16U + 2U * c + k / 2U + 8U * (k & 1U)) * L::kPitch + shift_of(b, 4U * c + k) + 2U * r;
 #pragma unroll
     for (int mt = 0; mt < HD / 16; ++mt) {
       uint32_t x[4];
@@ -621,10 +658,13 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
   __shared__ unsigned long long warp_units[kWarps];
   __shared__ uint32_t start_sequence;
   __shared__ unsigned long long start_base;
-  __shared__ float query_scale[4][kHeads];
   const uint32_t lane = threadIdx.x & 31U, warp = threadIdx.x >> 5U;
   const uint32_t capacity = kv_capacity(a.cache), sequences = a.cache.sequences;
-  const auto units_of = [&](uint32_t s) { return (min(a.lengths[s], capacity) + kUnit - 1U) / kUnit; };
+  // of one item of a sequence: its cost stands before its tokens in the line; nothing for a sequence without tokens
+  const auto units_of = [&](uint32_t s) {
+    const uint32_t n = (min(a.lengths[s], capacity) + kUnit - 1U) / kUnit;
+    return n ? n + plan.cost : 0U;
+  };
 
   // ---- this block's share [begin, end) of the line of units
   const uint32_t per_thread = (sequences + kThreads - 1U) / kThreads;
@@ -665,21 +705,23 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
   uint32_t s = start_sequence;
   unsigned long long base = start_base;
 
-  Warp<T, ENC, HD> w{a};
+  using W = Warp<T, ENC, HD>;
+  W w{a};
+  w.layout();
   w.lane = lane;
   w.r = lane >> 2U;
   w.c = lane & 3U;
   const uint32_t in_set = warp % plan.heads, phase = warp / plan.heads, phases = kWarps / plan.heads;
-  uint2* fragments = reinterpret_cast<uint2*>(shared);
-  uint8_t* area = shared + X::kFragmentBytes * plan.heads;
+  uint2* fragments = reinterpret_cast<uint2*>(shared + in_set * X::kQueryBytes);
+  uint8_t* area = shared + X::kQueryBytes * plan.heads;
   float* merge_max = reinterpret_cast<float*>(area);           // [warp][head]
   float* merge_sum = merge_max + kWarps * kHeads;
   float* merge_out = merge_sum + kWarps * kHeads;              // [warp][head][HD + 4]
-  w.fragments = fragments + in_set * (X::kFragmentBytes / sizeof(uint2));
+  w.fragments = fragments;
 
   while (u < end) {
     const uint32_t length = min(a.lengths[s], capacity);
-    const uint32_t n = (length + kUnit - 1U) / kUnit;
+    const uint32_t n = length ? (length + kUnit - 1U) / kUnit + plan.cost : 0U;
     if (u >= base + static_cast<unsigned long long>(n) * plan.items) {
       base += static_cast<unsigned long long>(n) * plan.items;
       ++s;
@@ -687,52 +729,81 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
     }
     const uint32_t item = static_cast<uint32_t>((u - base) / n), local = static_cast<uint32_t>((u - base) % n);
     const uint32_t take = static_cast<uint32_t>(min(static_cast<unsigned long long>(n - local), end - u));
-    const uint32_t first = local * kUnit, last = min(length, (local + take) * kUnit);
+    const uint32_t from = max(local, plan.cost) - plan.cost, upto = max(local + take, plan.cost) - plan.cost;  // units of tokens
+    if (from == upto) {  // the share ends before the item's first token
+      u += take;
+      continue;
+    }
+    const uint32_t first = from * kUnit, last = min(length, upto * kUnit);
     const uint32_t set = item / plan.tiles, tile = item % plan.tiles;
     const uint32_t heads_here = min(kHeads, plan.group - tile * kHeads);
     const uint32_t kv_head = set * plan.heads + in_set;
     const uint32_t head0 = kv_head * plan.group + tile * kHeads;  // first query head of this warp
 
-    // ---- the query heads as fragments (one warp per kv head), scaled to [2^8, 2^9)
-    __syncthreads();  // the merge area and the fragments of the item before have been read
-    if (warp < plan.heads) {
-      const T* q = static_cast<const T*>(a.query) + static_cast<size_t>(s) * a.query_stride + static_cast<size_t>(head0 + w.r) * HD;
-      const bool there = w.r < heads_here;
-      float top = 0.0F;
-      for (uint32_t d = w.c; d < HD; d += 4U) top = fmaxf(top, there ? fabsf(row_value(q[d])) : 0.0F);
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 2));
-      int up = 0;
-      if (top > 0.0F && top < INFINITY) up = 8 - ilogbf(top);
-      if (w.c == 0U) query_scale[warp][w.r] = ldexpf(a.scale * kLog2e, -up);
-      uint2* to = fragments + warp * (X::kFragmentBytes / sizeof(uint2));
-#pragma unroll 2
-      for (int step = 0; step < X::kSteps; ++step) {
-        uint32_t hi[2], lo[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          float x[2];
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-            x[half] = there ? ldexpf(row_value(q[L::query_dim(step, b, half, w.c)]), up) : 0.0F;
-          hi[b] = pack_half(x[0], x[1]);
-          const float2 f = unpack_half(hi[b]);
-          lo[b] = pack_half(x[0] - f.x, x[1] - f.y);
-        }
-        to[step * X::kTerms * 32 + lane] = make_uint2(hi[0], hi[1]);
-        if constexpr (X::kPrecise) to[(step * X::kTerms + 1) * 32 + lane] = make_uint2(lo[0], lo[1]);
-      }
-    }
-    __syncthreads();
-    uint2 q[X::kQueryInRegisters ? X::kSteps * X::kTerms : 1];
-    if constexpr (X::kQueryInRegisters) {
-#pragma unroll
-      for (int i = 0; i < X::kSteps * X::kTerms; ++i) q[i] = w.fragments[i * 32 + lane];
-    }
-    w.scale[0] = query_scale[in_set][2U * w.c];
-    w.scale[1] = query_scale[in_set][2U * w.c + 1U];
     w.sequence = s;
     w.kv_head = kv_head;
+    uint8_t* ring = area + warp * (L::kStages * L::kStage);
+    const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+    Cursor at(a.cache, first + 16U * (phase + phases * (L::kStaged ? 0U : lane % W::kN)), 16U * phases * W::kN);
+    typename W::Start x;
+    __syncthreads();  // the merge area and the queries of the item before have been read
+    // the first keys are on their way while the query is made ready (where it leaves room in the registers)
+    if constexpr (X::kQueryInRegisters) w.begin(x, at, first, last, phase, phases, ring_at);
+
+    // ---- the query heads as fragments, scaled to [2^8, 2^9)
+    constexpr uint32_t kChunks = kHeads * HD * sizeof(T) / 16U, kRowChunks = HD * sizeof(T) / 16U;
+    for (uint32_t i = threadIdx.x; i < plan.heads * kChunks; i += kThreads) {
+      const uint32_t h = i / kChunks, g = i % kChunks / kRowChunks, chunk = i % kRowChunks;
+      const T* q = static_cast<const T*>(a.query) + static_cast<size_t>(s) * a.query_stride +
+                   static_cast<size_t>((set * plan.heads + h) * plan.group + tile * kHeads + g) * HD;
+      *reinterpret_cast<uint4*>(shared + h * X::kQueryBytes + g * X::kQueryPitch + 16U * chunk) =
+          g < heads_here ? reinterpret_cast<const uint4*>(q)[chunk] : make_uint4(0U, 0U, 0U, 0U);
+    }
+    __syncthreads();
+    const T* row = reinterpret_cast<const T*>(shared + in_set * X::kQueryBytes + w.r * X::kQueryPitch);
+    float value[X::kSteps][2][2];
+    float top = 0.0F;
+#pragma unroll
+    for (int step = 0; step < X::kSteps; ++step)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          value[step][b][half] = row_value(row[L::query_dim(step, b, half, w.c)]);
+          top = fmaxf(top, fabsf(value[step][b][half]));
+        }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 2));
+    const int up = top > 0.0F && top < INFINITY ? 8 - ilogbf(top) : 0;
+    const float unit = ldexpf(a.scale * kLog2e, -up);  // of head r
+    w.scale[0] = __shfl_sync(0xffffffffU, unit, 8U * w.c);
+    w.scale[1] = __shfl_sync(0xffffffffU, unit, 8U * w.c + 4U);
+    // two factors: one may not be a float by itself
+    const float up0 = ldexpf(1.0F, up / 2), up1 = ldexpf(1.0F, up - up / 2);
+    uint2 q[X::kQueryInRegisters ? X::kSteps * X::kTerms : 1];
+    if constexpr (!X::kQueryInRegisters) __syncthreads();  // the fragments take the queries' place
+#pragma unroll
+    for (int step = 0; step < X::kSteps; ++step) {
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const float x0 = value[step][b][0] * up0 * up1, x1 = value[step][b][1] * up0 * up1;
+        hi[b] = pack_half(x0, x1);
+        const float2 f = unpack_half(hi[b]);
+        lo[b] = pack_half(x0 - f.x, x1 - f.y);
+      }
+      if constexpr (X::kQueryInRegisters) {
+        q[step * X::kTerms] = make_uint2(hi[0], hi[1]);
+        if constexpr (X::kPrecise) q[step * X::kTerms + 1] = make_uint2(lo[0], lo[1]);
+      } else if (phase == 0U) {
+        fragments[step * X::kTerms * 32 + lane] = make_uint2(hi[0], hi[1]);
+        if constexpr (X::kPrecise) fragments[(step * X::kTerms + 1) * 32 + lane] = make_uint2(lo[0], lo[1]);
+      }
+    }
+    if constexpr (!X::kQueryInRegisters) {
+      __syncthreads();
+      w.begin(x, at, first, last, phase, phases, ring_at);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       w.run.reference[h] = -INFINITY;
@@ -741,7 +812,7 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
       for (int mt = 0; mt < HD / 16; ++mt) w.run.out[mt][h] = w.run.out[mt][2 + h] = 0.0F;
     }
     float* scores = plan.scores ? plan.scores + (static_cast<size_t>(s) * a.q_heads + head0) * capacity : nullptr;
-    w.tokens(q, first, last, phase, phases, scores, capacity, heads_here, area + warp * (L::kStages * L::kStage));
+    w.tokens(x, at, q, first, last, phase, phases, scores, capacity, heads_here, ring);
 
     // ---- merge of the warps of one kv head
 #pragma unroll
@@ -761,9 +832,9 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
         *reinterpret_cast<float2*>(merge_out + row * X::kRow + L::out_dim(mt, w.r)) = make_float2(w.run.out[mt][h], w.run.out[mt][2 + h]);
     }
     __syncthreads();
-    const bool begins = local == 0U, whole = begins && take == n;
+    const bool begins = from == 0U, whole = begins && last == length;
     if (begins && threadIdx.x == 0U) {
-      const unsigned long long last_unit = u + n - 1ULL;
+      const unsigned long long last_unit = u - local + n - 1ULL;
       plan.spans[static_cast<size_t>(s) * plan.items + item] =
           make_uint2(blockIdx.x, static_cast<uint32_t>(((last_unit + 1ULL) * blocks - 1ULL) / total));
     }
@@ -786,11 +857,11 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
                 top == -INFINITY ? 0.0F : out / sum);
         if (plan.lse && d == 0U) plan.lse[static_cast<size_t>(s) * a.q_heads + head] = top == -INFINITY ? 0.0F : top + log2f(sum);
       } else {
-        float* to = place + static_cast<size_t>(h * kHeads + g) * (2U + HD);
-        to[2U + d] = out;
+        const uint32_t row = h * kHeads + g;
+        place[2U * plan.rows + row * HD + d] = out;
         if (d == 0U) {
-          to[0] = top;
-          to[1] = sum;
+          place[row] = top;
+          place[plan.rows + row] = sum;
         }
       }
     }
@@ -798,75 +869,137 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
   }
 }
 
-// One block per (sequence, query head): joins the parts of an item that lies in more than one share, and
-// writes the zeros of a sequence without tokens.
+// Second launch: blocks [0, sequences * q_heads) join, one query head each, the parts of an item that lies in more than
+// one share, and write the zeros of a sequence without tokens; the blocks behind them, `chunks` to a kv head, add the
+// weights of kWeightTokens tokens at a time.
+//
+// A joining warp takes every fourth part, a lane four dimensions of it; every lane works out the factors of the
+// parts it broadcasts, so that the only barrier is the one before the warps' sums are added.
+__device__ __forceinline__ const float* place_of(const Plan& plan, uint2 span, uint32_t i) {
+  return plan.partials + (static_cast<size_t>(span.x + i) * 2U + (i == 0U ? 1U : 0U)) * plan.place;
+}
+__device__ __forceinline__ uint2 span_of(const Plan& plan, uint32_t s, uint32_t kv_head, uint32_t g) {
+  return plan.spans[static_cast<size_t>(s) * plan.items + kv_head / plan.heads * plan.tiles + g / kHeads];
+}
+// Maximum over the parts (their reference, log2) and, in the lanes, parts of the sum.
+__device__ __forceinline__ float top_of(const Plan& plan, uint2 span, uint32_t row, uint32_t lane) {
+  float top = -INFINITY;
+  for (uint32_t i = lane; i < span.y - span.x + 1U; i += 32U) top = fmaxf(top, place_of(plan, span, i)[row]);
+  return warp_max(top);
+}
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ DecodeAttentionArgs a, const __grid_constant__ Plan plan) {
-  __shared__ float factor[kMaxBlocks], reduce[kJoinThreads / 32U], part[kJoinThreads];
-  pdl_wait();
-  const uint32_t head = blockIdx.x % a.q_heads, s = blockIdx.x / a.q_heads;
+__device__ __forceinline__ void join_head(const DecodeAttentionArgs& a, const Plan& plan, uint32_t s, uint32_t head) {
+  constexpr uint32_t kJoinWarps = kThreads / 32U;
+  constexpr uint32_t kVectors = (HD + 127) / 128;         // of four dimensions a lane holds
+  __shared__ float4 part[kJoinWarps][HD / 4];
   T* out = static_cast<T*>(a.out) + static_cast<size_t>(s) * a.out_stride + static_cast<size_t>(head) * HD;
   const uint32_t tid = threadIdx.x, lane = tid & 31U, warp = tid >> 5U;
   if (a.lengths[s] == 0U) {
-    if (tid < HD) put_row(out + tid, 0.0F);
+    for (uint32_t d = tid; d < HD; d += kThreads) put_row(out + d, 0.0F);
     return;
   }
   const uint32_t kv_head = head / plan.group, g = head % plan.group;
-  const uint2 span = plan.spans[static_cast<size_t>(s) * plan.items + kv_head / plan.heads * plan.tiles + g / kHeads];
+  const uint2 span = span_of(plan, s, kv_head, g);
   const uint32_t count = span.y - span.x + 1U;
   if (count <= 1U) return;
-  const float* parts = plan.partials + static_cast<size_t>((kv_head % plan.heads) * kHeads + g % kHeads) * (2U + HD);
-  const auto part_of = [&](uint32_t i) { return parts + (static_cast<size_t>(span.x + i) * 2U + (i == 0U ? 1U : 0U)) * plan.place; };
-  float top = -INFINITY;
-  for (uint32_t i = tid; i < count; i += kJoinThreads) top = fmaxf(top, part_of(i)[0]);
-  top = warp_max(top);
-  if (lane == 0U) reduce[warp] = top;
-  __syncthreads();
-  top = reduce[0];
-#pragma unroll
-  for (uint32_t w = 1; w < kJoinThreads / 32U; ++w) top = fmaxf(top, reduce[w]);
+  const uint32_t row = (kv_head % plan.heads) * kHeads + g % kHeads;
+  const float top = top_of(plan, span, row, lane);
+  const float reference = top == -INFINITY ? 0.0F : top;
   float sum = 0.0F;
-  for (uint32_t i = tid; i < count; i += kJoinThreads) {
-    const float f = top == -INFINITY ? 0.0F : exp2_fast(part_of(i)[0] - top);
-    factor[i] = f;
-    sum += part_of(i)[1] * f;
+  float4 acc[kVectors];
+#pragma unroll
+  for (uint32_t v = 0; v < kVectors; ++v) acc[v] = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+  for (uint32_t i0 = 0; i0 < count; i0 += 32U) {  // 32 parts: lane i has the factor of part i0 + i, each warp adds eight
+    const bool there = i0 + lane < count;
+    const float factor = there ? exp2_fast(place_of(plan, span, i0 + lane)[row] - reference) : 0.0F;
+    sum += there ? place_of(plan, span, i0 + lane)[plan.rows + row] * factor : 0.0F;
+#pragma unroll
+    for (uint32_t j = 0; j < 32U / kJoinWarps; ++j) {
+      const uint32_t i = j * kJoinWarps + warp;
+      const float f = __shfl_sync(0xffffffffU, factor, i);
+      if (i0 + i >= count) continue;
+      const float4* from = reinterpret_cast<const float4*>(place_of(plan, span, i0 + i) + 2U * plan.rows + row * HD);
+#pragma unroll
+      for (uint32_t v = 0; v < kVectors; ++v) {
+        if (lane + 32U * v >= HD / 4) continue;
+        const float4 x = from[lane + 32U * v];
+        acc[v].x = fmaf(x.x, f, acc[v].x);
+        acc[v].y = fmaf(x.y, f, acc[v].y);
+        acc[v].z = fmaf(x.z, f, acc[v].z);
+        acc[v].w = fmaf(x.w, f, acc[v].w);
+      }
+    }
   }
   sum = warp_sum(sum);
-  __syncthreads();
-  if (lane == 0U) reduce[warp] = sum;
-  __syncthreads();
-  sum = 0.0F;
 #pragma unroll
-  for (uint32_t w = 0; w < kJoinThreads / 32U; ++w) sum += reduce[w];
-  constexpr uint32_t kWays = kJoinThreads / HD;  // 4, 2, 1, 1
-  const uint32_t d = tid % HD, way = tid / HD;
-  float acc = 0.0F;
-  if (way < kWays)
-#pragma unroll 4
-    for (uint32_t i = way; i < count; i += kWays) acc = fmaf(part_of(i)[2U + d], factor[i], acc);
-  part[tid] = acc;
+  for (uint32_t v = 0; v < kVectors; ++v)
+    if (lane + 32U * v < HD / 4) part[warp][lane + 32U * v] = acc[v];
   __syncthreads();
-  if (tid < HD) {
+  for (uint32_t d = tid; d < HD; d += kThreads) {
+    float total = 0.0F;
 #pragma unroll
-    for (uint32_t w = 1; w < kWays; ++w) acc += part[w * HD + tid];
-    put_row(out + tid, top == -INFINITY ? 0.0F : acc / sum);
+    for (uint32_t w = 0; w < kJoinWarps; ++w) total += reinterpret_cast<const float*>(part[w])[d];
+    put_row(out + d, top == -INFINITY ? 0.0F : total / sum);
   }
-  if (plan.lse && tid == 0U) plan.lse[static_cast<size_t>(s) * a.q_heads + head] = top == -INFINITY ? 0.0F : top + log2f(sum);
 }
 
-// grid (sequences * kv heads, chunks of slots)
-__global__ void __launch_bounds__(kThreads) decode_weights_kernel(const __grid_constant__ DecodeAttentionArgs a, const __grid_constant__ Plan plan) {
-  pdl_wait();
-  const uint32_t s = blockIdx.x / a.cache.kv_heads, h = blockIdx.x % a.cache.kv_heads;
+__device__ __forceinline__ void add_weights(const DecodeAttentionArgs& a, const Plan& plan, uint32_t s, uint32_t h, uint32_t chunk, uint32_t chunks) {
+  __shared__ float lse[kHeads];
+  const uint32_t lane = threadIdx.x & 31U, warp = threadIdx.x >> 5U;
   const uint32_t capacity = kv_capacity(a.cache), n = min(a.lengths[s], capacity);
-  const float* lse = plan.lse + static_cast<size_t>(s) * a.q_heads + h * plan.group;
-  const float* scores = plan.scores + (static_cast<size_t>(s) * a.q_heads + h * plan.group) * capacity;
-  const size_t row = static_cast<size_t>(blockIdx.x) * a.weights_stride;
-  for (uint32_t t = blockIdx.y * kThreads + threadIdx.x; t < n; t += gridDim.y * kThreads) {
-    float sum = 0.0F;
-    for (uint32_t g = 0; g < plan.group; ++g) sum += exp2_fast(scores[g * static_cast<size_t>(capacity) + t] - lse[g]);
-    a.weights_out[row + t] = (a.weights_in ? a.weights_in[row + t] : 0.0F) + sum;
+  const size_t row = (static_cast<size_t>(s) * a.cache.kv_heads + h) * a.weights_stride;
+  for (uint32_t t0 = chunk * kWeightTokens; t0 < n; t0 += chunks * kWeightTokens) {
+    float sum[kWeightTokens / kThreads] = {};
+    for (uint32_t g0 = 0; g0 < plan.group; g0 += kHeads) {
+      const uint32_t here = min(kHeads, plan.group - g0);
+      const uint32_t head0 = h * plan.group + g0;
+      const uint2 span = span_of(plan, s, h, g0);
+      __syncthreads();
+      for (uint32_t g = warp; g < here; g += kThreads / 32U) {
+        float value;
+        if (span.x == span.y) {
+          value = plan.lse[static_cast<size_t>(s) * a.q_heads + head0 + g];
+        } else {
+          const uint32_t place_row = (h % plan.heads) * kHeads + g;
+          const float top = top_of(plan, span, place_row, lane);
+          float total = 0.0F;
+          if (top != -INFINITY)
+            for (uint32_t i = lane; i < span.y - span.x + 1U; i += 32U)
+              total += place_of(plan, span, i)[plan.rows + place_row] * exp2_fast(place_of(plan, span, i)[place_row] - top);
+          total = warp_sum(total);
+          value = top == -INFINITY ? 0.0F : top + log2f(total);
+        }
+        if (lane == 0U) lse[g] = value;
+      }
+      __syncthreads();
+      const float* scores = plan.scores + (static_cast<size_t>(s) * a.q_heads + head0) * capacity;
+#pragma unroll 2
+      for (uint32_t g = 0; g < here; ++g)
+#pragma unroll
+        for (uint32_t i = 0; i < kWeightTokens / kThreads; ++i) {
+          const uint32_t t = t0 + i * kThreads + threadIdx.x;
+          if (t < n) sum[i] += exp2_fast(scores[static_cast<size_t>(g) * capacity + t] - lse[g]);
+        }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kWeightTokens / kThreads; ++i) {
+      const uint32_t t = t0 + i * kThreads + threadIdx.x;
+      if (t < n) a.weights_out[row + t] = (a.weights_in ? a.weights_in[row + t] : 0.0F) + sum[i];
+    }
   }
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_constant__ DecodeAttentionArgs a, const __grid_constant__ Plan plan, uint32_t chunks) {
+  pdl_wait();
+  const uint32_t joins = a.cache.sequences * a.q_heads;
+  if (blockIdx.x < joins) {
+    join_head<T, HD>(a, plan, blockIdx.x / a.q_heads, blockIdx.x % a.q_heads);
+    return;
+  }
+  const uint32_t row = (blockIdx.x - joins) / chunks, chunk = (blockIdx.x - joins) % chunks;
+  add_weights(a, plan, row / a.cache.kv_heads, row % a.cache.kv_heads, chunk, chunks);
 }
 
 int multiprocessors(uint32_t* count) {
@@ -887,16 +1020,17 @@ int launch(const DecodeAttentionArgs& a, const Plan& plan, cudaStream_t stream) 
                                        static_cast<int>(X::kShared)), "decode_attention shared memory opt-in");
   if (rc) return rc;
   const uint32_t grid = min(kMaxBlocks, sms * X::kBlocksPerSm);
-  count_launch(plan.scores ? 3U : 2U);
+  count_launch(2U);
   rc = check_cuda(launch_ordered(decode_attention_kernel<T, ENC, HD>, dim3(grid), dim3(kThreads), X::kShared, stream, a, plan),
                   "decode_attention");
   if (rc) return rc;
-  rc = check_cuda(launch_pdl(decode_join_kernel<T, HD>, dim3(a.cache.sequences * a.q_heads), dim3(kJoinThreads), 0, stream, a, plan),
-                  "decode_attention join");
-  if (rc || !plan.scores) return rc;
-  const uint32_t rows = a.cache.sequences * a.cache.kv_heads;
-  const uint32_t chunks = min(256U, (kv_capacity(a.cache) + kThreads - 1U) / kThreads);
-  return check_cuda(launch_pdl(decode_weights_kernel, dim3(rows, chunks), dim3(kThreads), 0, stream, a, plan), "decode_attention weights");
+  uint32_t blocks = a.cache.sequences * a.q_heads, chunks = 1U;
+  if (plan.scores) {
+    const uint32_t rows = a.cache.sequences * a.cache.kv_heads;
+    chunks = min(min(256U, (kv_capacity(a.cache) + kWeightTokens - 1U) / kWeightTokens), max(1U, (1U << 30U) / rows));
+    blocks += rows * chunks;
+  }
+  return check_cuda(launch_pdl(decode_join_kernel<T, HD>, dim3(blocks), dim3(kThreads), 0, stream, a, plan, chunks), "decode_attention join");
 }
 
 template <typename T, int ENC>
