@@ -155,7 +155,8 @@ __device__ __forceinline__ void nibbles_to_half(uint32_t w, uint32_t (&h)[4]) {
   h[2] = half2_sub(mask_flip<0x000F000FU, 0x64086408U>(high), 0x64086408U);
   h[3] = half2_fma(mask_flip<0x00F000F0U, 0x64806480U>(high), 0x2C002C00U, 0xD480D480U);
 }
-// Signed bytes in bits 0-7 of each half -> F16: 0x6400 | (b ^ 0x80) is 1024 + b + 128.
+// Signed bytes in bits 0-7 of each half -> F16: 0x6400 | (b ^ 0x80) is 1024 + b + 128.  (Left in, and the sum of the weights times
+// 1152 taken off at the end, V's bias would cost FP32 sums four bits.)
 __device__ __forceinline__ uint32_t bytes_to_half(uint32_t v) {
   return half2_sub(mask_flip<0x00FF00FFU, 0x64806480U>(v), 0x64806480U);
 }
@@ -468,18 +469,22 @@ struct Warp {
   }
 
   // ---- through shared memory (Q8): rows of windows, key 2r in row r, key 2r + 1 in row r + 8
+  // The windows of the keys one after the other over the lanes: 144 bytes in a row of one key (four lanes to a key and
+  // eight keys at a time need fewer instructions, but fetch a sector twice more often: 152 us against 144 us).
   __device__ __forceinline__ void stage(const Block& b, uint32_t to) {
     constexpr int kCopies = (16 * L::kWindows + 31) / 32;  // of a lane, for K and for V
     const uint8_t* base = b.keys ? b.keys : reinterpret_cast<const uint8_t*>(a.cache.page_tables);
+    const uint32_t step = b.keys ? stride : 0U, to_v = b.keys ? to_values : 0U;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
       const uint32_t index = lane + 32U * i, key = index / L::kWindows, window = index % L::kWindows;
       if (index >= 16U * L::kWindows) break;
-      const uintptr_t record = reinterpret_cast<uintptr_t>(base) + (b.keys ? key * stride : 0U);
-      const uint8_t* from = reinterpret_cast<const uint8_t*>(record & ~static_cast<uintptr_t>(15U)) + 16U * window;
-      const uint32_t row = key / 2U + 8U * (key & 1U);
-      copy16(to + row * L::kPitch + 16U * window, from, key < b.count);
-      copy16(to + (16U + row) * L::kPitch + 16U * window, from + (b.keys ? to_values : 0U), key < b.count);  // V begins on 16 bytes
+      const bool there = key < b.count;  // else zeros, and the address only has to be one that exists
+      const uint8_t* from =
+          reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(base + key * step) & ~static_cast<uintptr_t>(15U)) + 16U * window;
+      const uint32_t row = to + (key / 2U + 8U * (key & 1U)) * L::kPitch + 16U * window;
+      copy16(row, from, there);
+      copy16(row + 16U * L::kPitch, from + to_v, there);  // V begins on 16 bytes
     }
   }
   // where a record begins in its row (K and V alike; pages and layers begin on 16 bytes)
@@ -869,12 +874,11 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
   }
 }
 
-// Second launch: blocks [0, sequences * q_heads) join, one query head each, the parts of an item that lies in more than
-// one share, and write the zeros of a sequence without tokens; the blocks behind them, `chunks` to a kv head, add the
-// weights of kWeightTokens tokens at a time.
-//
-// A joining warp takes every fourth part, a lane four dimensions of it; every lane works out the factors of the
-// parts it broadcasts, so that the only barrier is the one before the warps' sums are added.
+// Second launch.  Its last blocks join the parts of the items that lie in more than one share, and write the zeros of
+// the sequences without tokens: kWays warps to a query head, four (the warps of a block; long sequences of many parts) or one (many
+// sequences of few parts: a block per head costs a chain of four loads for two or three parts).  A warp takes every
+// kWays-th part, a lane four dimensions of it, and every lane works out the factors of the parts it broadcasts.
+// The blocks before them, `chunks` to a kv head, add up the weights: scores and log-sums are in the workspace.
 __device__ __forceinline__ const float* place_of(const Plan& plan, uint2 span, uint32_t i) {
   return plan.partials + (static_cast<size_t>(span.x + i) * 2U + (i == 0U ? 1U : 0U)) * plan.place;
 }
@@ -888,15 +892,14 @@ __device__ __forceinline__ float top_of(const Plan& plan, uint2 span, uint32_t r
   return warp_max(top);
 }
 
-template <typename T, int HD>
-__device__ __forceinline__ void join_head(const DecodeAttentionArgs& a, const Plan& plan, uint32_t s, uint32_t head) {
-  constexpr uint32_t kJoinWarps = kThreads / 32U;
+template <typename T, int HD, uint32_t kWays>
+__device__ __forceinline__ void join_head(const DecodeAttentionArgs& a, const Plan& plan, uint32_t s, uint32_t head, uint32_t way) {
   constexpr uint32_t kVectors = (HD + 127) / 128;         // of four dimensions a lane holds
-  __shared__ float4 part[kJoinWarps][HD / 4];
+  __shared__ float4 part[kWays > 1U ? kWays : 1U][kWays > 1U ? HD / 4 : 1];
   T* out = static_cast<T*>(a.out) + static_cast<size_t>(s) * a.out_stride + static_cast<size_t>(head) * HD;
-  const uint32_t tid = threadIdx.x, lane = tid & 31U, warp = tid >> 5U;
+  const uint32_t lane = threadIdx.x & 31U;
   if (a.lengths[s] == 0U) {
-    for (uint32_t d = tid; d < HD; d += kThreads) put_row(out + d, 0.0F);
+    for (uint32_t d = way * 32U + lane; d < HD; d += 32U * kWays) put_row(out + d, 0.0F);
     return;
   }
   const uint32_t kv_head = head / plan.group, g = head % plan.group;
@@ -910,15 +913,14 @@ __device__ __forceinline__ void join_head(const DecodeAttentionArgs& a, const Pl
   float4 acc[kVectors];
 #pragma unroll
   for (uint32_t v = 0; v < kVectors; ++v) acc[v] = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-  for (uint32_t i0 = 0; i0 < count; i0 += 32U) {  // 32 parts: lane i has the factor of part i0 + i, each warp adds eight
+  for (uint32_t i0 = 0; i0 < count; i0 += 32U) {  // 32 parts: lane i has the factor of part i0 + i, each warp adds its own
     const bool there = i0 + lane < count;
     const float factor = there ? exp2_fast(place_of(plan, span, i0 + lane)[row] - reference) : 0.0F;
     sum += there ? place_of(plan, span, i0 + lane)[plan.rows + row] * factor : 0.0F;
-#pragma unroll
-    for (uint32_t j = 0; j < 32U / kJoinWarps; ++j) {
-      const uint32_t i = j * kJoinWarps + warp;
+    const uint32_t here = min(32U, count - i0);
+#pragma unroll 8
+    for (uint32_t i = way; i < here; i += kWays) {
       const float f = __shfl_sync(0xffffffffU, factor, i);
-      if (i0 + i >= count) continue;
       const float4* from = reinterpret_cast<const float4*>(place_of(plan, span, i0 + i) + 2U * plan.rows + row * HD);
 #pragma unroll
       for (uint32_t v = 0; v < kVectors; ++v) {
@@ -932,74 +934,101 @@ __device__ __forceinline__ void join_head(const DecodeAttentionArgs& a, const Pl
     }
   }
   sum = warp_sum(sum);
+  if constexpr (kWays > 1U) {
 #pragma unroll
-  for (uint32_t v = 0; v < kVectors; ++v)
-    if (lane + 32U * v < HD / 4) part[warp][lane + 32U * v] = acc[v];
-  __syncthreads();
-  for (uint32_t d = tid; d < HD; d += kThreads) {
-    float total = 0.0F;
+    for (uint32_t v = 0; v < kVectors; ++v)
+      if (lane + 32U * v < HD / 4) part[way][lane + 32U * v] = acc[v];
+    __syncthreads();
+    for (uint32_t d = way * 32U + lane; d < HD; d += 32U * kWays) {
+      float total = 0.0F;
 #pragma unroll
-    for (uint32_t w = 0; w < kJoinWarps; ++w) total += reinterpret_cast<const float*>(part[w])[d];
-    put_row(out + d, top == -INFINITY ? 0.0F : total / sum);
+      for (uint32_t w = 0; w < kWays; ++w) total += reinterpret_cast<const float*>(part[w])[d];
+      put_row(out + d, top == -INFINITY ? 0.0F : total / sum);
+    }
+  } else {
+    const float scale = top == -INFINITY ? 0.0F : 1.0F / sum;
+#pragma unroll
+    for (uint32_t v = 0; v < kVectors; ++v) {
+      if (lane + 32U * v >= HD / 4) continue;
+      T* to = out + 4U * (lane + 32U * v);
+      put_row(to, acc[v].x * scale);
+      put_row(to + 1, acc[v].y * scale);
+      put_row(to + 2, acc[v].z * scale);
+      put_row(to + 3, acc[v].w * scale);
+    }
   }
 }
 
 __device__ __forceinline__ void add_weights(const DecodeAttentionArgs& a, const Plan& plan, uint32_t s, uint32_t h, uint32_t chunk, uint32_t chunks) {
   __shared__ float lse[kHeads];
+  constexpr uint32_t kEach = kWeightTokens / kThreads;
   const uint32_t lane = threadIdx.x & 31U, warp = threadIdx.x >> 5U;
   const uint32_t capacity = kv_capacity(a.cache), n = min(a.lengths[s], capacity);
+  if (chunk * kWeightTokens >= n) return;
   const size_t row = (static_cast<size_t>(s) * a.cache.kv_heads + h) * a.weights_stride;
-  for (uint32_t t0 = chunk * kWeightTokens; t0 < n; t0 += chunks * kWeightTokens) {
-    float sum[kWeightTokens / kThreads] = {};
-    for (uint32_t g0 = 0; g0 < plan.group; g0 += kHeads) {
-      const uint32_t here = min(kHeads, plan.group - g0);
-      const uint32_t head0 = h * plan.group + g0;
-      const uint2 span = span_of(plan, s, h, g0);
-      __syncthreads();
-      for (uint32_t g = warp; g < here; g += kThreads / 32U) {
-        float value;
-        if (span.x == span.y) {
-          value = plan.lse[static_cast<size_t>(s) * a.q_heads + head0 + g];
-        } else {
-          const uint32_t place_row = (h % plan.heads) * kHeads + g;
-          const float top = top_of(plan, span, place_row, lane);
-          float total = 0.0F;
-          if (top != -INFINITY)
-            for (uint32_t i = lane; i < span.y - span.x + 1U; i += 32U)
-              total += place_of(plan, span, i)[plan.rows + place_row] * exp2_fast(place_of(plan, span, i)[place_row] - top);
-          total = warp_sum(total);
-          value = top == -INFINITY ? 0.0F : top + log2f(total);
-        }
-        if (lane == 0U) lse[g] = value;
+  for (uint32_t g0 = 0; g0 < plan.group; g0 += kHeads) {
+    const uint32_t here = min(kHeads, plan.group - g0);
+    const uint32_t head0 = h * plan.group + g0;
+    const uint2 span = span_of(plan, s, h, g0);
+    __syncthreads();
+    for (uint32_t g = warp; g < here; g += kThreads / 32U) {
+      float value;
+      if (span.x == span.y) {
+        value = plan.lse[static_cast<size_t>(s) * a.q_heads + head0 + g];
+      } else {
+        const uint32_t place_row = (h % plan.heads) * kHeads + g;
+        const float top = top_of(plan, span, place_row, lane);
+        float total = 0.0F;
+        if (top != -INFINITY)
+          for (uint32_t i = lane; i < span.y - span.x + 1U; i += 32U)
+            total += place_of(plan, span, i)[plan.rows + place_row] * exp2_fast(place_of(plan, span, i)[place_row] - top);
+        total = warp_sum(total);
+        value = top == -INFINITY ? 0.0F : top + log2f(total);
       }
-      __syncthreads();
-      const float* scores = plan.scores + (static_cast<size_t>(s) * a.q_heads + head0) * capacity;
-#pragma unroll 2
-      for (uint32_t g = 0; g < here; ++g)
-#pragma unroll
-        for (uint32_t i = 0; i < kWeightTokens / kThreads; ++i) {
-          const uint32_t t = t0 + i * kThreads + threadIdx.x;
-          if (t < n) sum[i] += exp2_fast(scores[static_cast<size_t>(g) * capacity + t] - lse[g]);
-        }
+      if (lane == 0U) lse[g] = value;
     }
+    __syncthreads();
+    const float* scores = plan.scores + (static_cast<size_t>(s) * a.q_heads + head0) * capacity;
+    const float* start = g0 ? a.weights_out : a.weights_in;
+    for (uint32_t t0 = chunk * kWeightTokens; t0 < n; t0 += chunks * kWeightTokens) {
+      float before[kEach], score[kHeads][kEach];
 #pragma unroll
-    for (uint32_t i = 0; i < kWeightTokens / kThreads; ++i) {
-      const uint32_t t = t0 + i * kThreads + threadIdx.x;
-      if (t < n) a.weights_out[row + t] = (a.weights_in ? a.weights_in[row + t] : 0.0F) + sum[i];
+      for (uint32_t i = 0; i < kEach; ++i) {
+        const uint32_t t = t0 + i * kThreads + threadIdx.x;
+        before[i] = start && t < n ? start[row + t] : 0.0F;
+#pragma unroll
+        for (uint32_t g = 0; g < kHeads; ++g) score[g][i] = g < here && t < n ? scores[static_cast<size_t>(g) * capacity + t] : -INFINITY;
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < kEach; ++i) {
+        const uint32_t t = t0 + i * kThreads + threadIdx.x;
+        float added = 0.0F;
+#pragma unroll
+        for (uint32_t g = 0; g < kHeads; ++g)
+          if (g < here) added += exp2_fast(score[g][i] - lse[g]);
+        if (t < n) a.weights_out[row + t] = before[i] + added;
+      }
     }
   }
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_constant__ DecodeAttentionArgs a, const __grid_constant__ Plan plan, uint32_t chunks) {
+__global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_constant__ DecodeAttentionArgs a, const __grid_constant__ Plan plan,
+                                                               uint32_t joins, uint32_t ways, uint32_t chunks) {
   pdl_wait();
-  const uint32_t joins = a.cache.sequences * a.q_heads;
-  if (blockIdx.x < joins) {
-    join_head<T, HD>(a, plan, blockIdx.x / a.q_heads, blockIdx.x % a.q_heads);
+  const uint32_t warp = threadIdx.x >> 5U, first_join = gridDim.x - joins;
+  if (blockIdx.x < first_join) {
+    const uint32_t row = blockIdx.x / chunks;
+    add_weights(a, plan, row / a.cache.kv_heads, row % a.cache.kv_heads, blockIdx.x % chunks, chunks);
     return;
   }
-  const uint32_t row = (blockIdx.x - joins) / chunks, chunk = (blockIdx.x - joins) % chunks;
-  add_weights(a, plan, row / a.cache.kv_heads, row % a.cache.kv_heads, chunk, chunks);
+  const uint32_t block = blockIdx.x - first_join;
+  if (ways == kWarps) {
+    join_head<T, HD, kWarps>(a, plan, block / a.q_heads, block % a.q_heads, warp);
+  } else {
+    const uint32_t head = block * kWarps + warp;
+    if (head < a.cache.sequences * a.q_heads) join_head<T, HD, 1>(a, plan, head / a.q_heads, head % a.q_heads, 0U);
+  }
 }
 
 int multiprocessors(uint32_t* count) {
@@ -1024,13 +1053,17 @@ int launch(const DecodeAttentionArgs& a, const Plan& plan, cudaStream_t stream) 
   rc = check_cuda(launch_ordered(decode_attention_kernel<T, ENC, HD>, dim3(grid), dim3(kThreads), X::kShared, stream, a, plan),
                   "decode_attention");
   if (rc) return rc;
-  uint32_t blocks = a.cache.sequences * a.q_heads, chunks = 1U;
-  if (plan.scores) {
-    const uint32_t rows = a.cache.sequences * a.cache.kv_heads;
-    chunks = min(min(256U, (kv_capacity(a.cache) + kWeightTokens - 1U) / kWeightTokens), max(1U, (1U << 30U) / rows));
-    blocks += rows * chunks;
+  // four warps to a query head as long as they find room at once
+  const uint32_t heads = a.cache.sequences * a.q_heads;
+  const uint32_t ways = heads <= 8U * sms ? kWarps : 1U;
+  const uint32_t joins = ways == kWarps ? heads : (heads + kWarps - 1U) / kWarps;
+  uint32_t chunks = 1U, rows = 0U;
+  if (plan.scores) {  // about 16 blocks to a multiprocessor (4: 170 us, 8: 164 us, 16: 163 us for 96 ragged sequences)
+    rows = a.cache.sequences * a.cache.kv_heads;
+    chunks = max(1U, min((16U * sms + rows - 1U) / rows, (kv_capacity(a.cache) + kWeightTokens - 1U) / kWeightTokens));
   }
-  return check_cuda(launch_pdl(decode_join_kernel<T, HD>, dim3(blocks), dim3(kThreads), 0, stream, a, plan, chunks), "decode_attention join");
+  return check_cuda(launch_pdl(decode_join_kernel<T, HD>, dim3(joins + rows * chunks), dim3(kThreads), 0, stream, a, plan, joins, ways, chunks),
+                    "decode_attention join");
 }
 
 template <typename T, int ENC>

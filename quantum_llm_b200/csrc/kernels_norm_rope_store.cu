@@ -11,8 +11,11 @@
 //
 // HBM-bound: a row is read once and its results written once.  A lane owns the eight values at i and
 // the eight at i + R/2 (the pair that a rotation mixes), so a head of 128 is eight lanes with two
-// 16-byte loads each, a warp takes four heads at a time, no value crosses lanes except in the sum of
-// squares (and the maximum of a quantised record), and nothing but cos and sin is in shared memory.
+// 16-byte loads each, a warp takes four heads at a time and no value crosses lanes except in the sum of
+// squares (and the maximum of a quantised record).  A warp takes a whole row, or, where rows are few, some heads
+// of one: its lanes share the work of the cosines and sines and hand them round by shuffles, so that
+// warps need no barrier, and the values of the next passes are copied into shared memory (each lane its own)
+// while these are worked on.
 #include "kv_batch.cuh"
 #include "launch.cuh"
 
@@ -21,6 +24,7 @@ namespace qllm {
 namespace {
 
 constexpr uint32_t kThreads = 256;
+constexpr uint32_t kWarpsWanted = 4096;  // of a launch
 
 template <int kLanes>
 __device__ __forceinline__ float head_sum(float v) {
@@ -64,117 +68,169 @@ __device__ __forceinline__ void store_record8(const KvBatch& c, uint8_t* codes, 
   }
 }
 
-// grid (rows, blocks of heads)
-template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads)
-norm_rope_store_kernel(NormRopeStoreArgs a, uint32_t heads_per_block) {
-  constexpr int kActive = HD / 16;                        // lanes that hold a head
-  constexpr int kLanes = kActive == 12 ? 16 : kActive;    // lanes set aside for it
-  constexpr uint32_t kHeadsPerWarp = 32 / kLanes;
-  __shared__ float2 turn[HD / 2];                         // cos, sin
-  const uint32_t row = blockIdx.x;
-  const uint32_t slot = a.row_slot ? a.row_slot[row] : 0U;
-  if (slot == kPaddingSlot) return;
-  const uint32_t position = a.positions[row];
-  for (uint32_t i = threadIdx.x; i < a.rotary_dim / 2U; i += kThreads) {
-    double t = static_cast<double>(position) * static_cast<double>(a.inv_freq[i]) * 0.15915494309189533577;
-    t -= rint(t);  // turns, in [-1/2, 1/2]
-    float s, c;
-    sincospif(2.0F * static_cast<float>(t), &s, &c);
-    turn[i] = make_float2(c, s);
-  }
-  const uint32_t sequence = a.row_sequence ? a.row_sequence[row] : row;
-  uint8_t* layer = nullptr;
-  if (a.row_slot && sequence < a.cache.sequences && slot < kv_capacity(a.cache))
-    layer = kv_page(a.cache, sequence, slot / a.cache.page_tokens);
-  const uint32_t place = slot % a.cache.page_tokens;
-  __syncthreads();
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
 
-  const uint32_t kv = a.cache.kv_heads;
-  const uint32_t first = blockIdx.y * heads_per_block;
-  const uint32_t all = a.q_heads + (a.row_slot ? 2U : 1U) * kv;
-  const uint32_t last = min(all, first + heads_per_block);
-  const uint32_t lane = threadIdx.x & 31U, warp = threadIdx.x >> 5U;
-  const uint32_t l = lane % kLanes;
-  const bool holds = l < kActive;
+// One warp per task: `passes` times kHeadsPerWarp heads of one row.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 4)
+norm_rope_store_kernel(const __grid_constant__ NormRopeStoreArgs a, uint32_t tasks_per_row, uint32_t passes) {
+  constexpr uint32_t kActive = HD / 16;                        // lanes that hold a head
+  constexpr uint32_t kLanes = kActive == 12U ? 16U : kActive;  // lanes set aside for it
+  constexpr uint32_t kHeadsPerWarp = 32U / kLanes;
+  constexpr uint32_t kTurns = kLanes / 4U;                     // cosines a lane works out
+  constexpr uint32_t kStages = sizeof(T) == 2U ? 4U : 2U;      // passes in flight: 32 KiB of a block
+  constexpr uint32_t kWords = sizeof(T) / 2U;                  // 16-byte words of eight values
+  __shared__ alignas(16) float norm[2][HD];
+  __shared__ uint4 ring[kStages][2U * kWords][kThreads];       // a lane's values of the passes to come; nobody else reads them
+  for (uint32_t i = threadIdx.x; i < 2U * HD; i += kThreads) norm[i / HD][i % HD] = (i < HD ? a.q_norm : a.k_norm)[i % HD];
+  __syncthreads();
+  const uint64_t task = static_cast<uint64_t>(blockIdx.x) * (kThreads / 32U) + (threadIdx.x >> 5U);
+  const uint32_t row = static_cast<uint32_t>(task / tasks_per_row);
+  if (row >= a.rows) return;
+  const uint32_t lane = threadIdx.x & 31U, l = lane % kLanes, which = lane / kLanes;
+  const uint32_t kv = a.cache.kv_heads, all = a.q_heads + (a.row_slot ? 2U : 1U) * kv;
+  const uint32_t first = static_cast<uint32_t>(task % tasks_per_row) * passes * kHeadsPerWarp;
+  const uint32_t last = min(all, first + passes * kHeadsPerWarp);
   // chunks of eight values: the pair (l, l + R/16) inside the rotation, two neighbours outside
   const uint32_t turned = a.rotary_dim / 16U;
   const bool rotates = l < turned;
   const uint32_t c0 = rotates ? l : a.rotary_dim / 8U + 2U * (l - turned);
   const uint32_t c1 = rotates ? l + turned : c0 + 1U;
   const T* x = static_cast<const T*>(a.qkv) + static_cast<size_t>(row) * a.qkv_stride;
-
-  for (uint32_t base = first + warp * kHeadsPerWarp; base < last; base += (kThreads / 32U) * kHeadsPerWarp) {
-    const uint32_t head = base + lane / kLanes;
-    const bool live = holds && head < last;
-    float v0[8] = {}, v1[8] = {};
-    if (live) {
-      load8(x + static_cast<size_t>(head) * HD + 8U * c0, v0);
-      load8(x + static_cast<size_t>(head) * HD + 8U * c1, v1);
-    }
-    const bool is_value = head >= a.q_heads + kv;
-    float sum = 0.0F;
+  const auto fetch = [&](uint32_t head, uint32_t stage) {
+    if (l < kActive && head < last) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(v0[i], v0[i], fmaf(v1[i], v1[i], sum));
-    sum = head_sum<kLanes>(sum);
-    if (live && !is_value) {
-      const float* w = head < a.q_heads ? a.q_norm : a.k_norm;
-      const float r = 1.0F / sqrtf(sum / static_cast<float>(HD) + a.eps);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v0[i] = v0[i] * r * w[8U * c0 + i];
-        v1[i] = v1[i] * r * w[8U * c1 + i];
+      for (uint32_t i = 0; i < kWords; ++i) {
+        copy16(&ring[stage][i][threadIdx.x], x + static_cast<size_t>(head) * HD + 8U * c0 + i * 16U / sizeof(T));
+        copy16(&ring[stage][kWords + i][threadIdx.x], x + static_cast<size_t>(head) * HD + 8U * c1 + i * 16U / sizeof(T));
       }
-      if (rotates) {
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (uint32_t i = 0; i < kStages - 1U; ++i) fetch(first + i * kHeadsPerWarp + which, i);
+
+  const uint32_t slot = a.row_slot ? a.row_slot[row] : 0U;
+  if (slot == kPaddingSlot) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");  // its copies are not to outlive the block
+    return;
+  }
+  const uint32_t position = a.positions[row];
+  const uint32_t sequence = a.row_sequence ? a.row_sequence[row] : row;
+  // cos and sin of the lane's pairs 8 l .. 8 l + 7: the lanes of the kHeadsPerWarp heads work out kTurns of them each
+  float cosine[8], sine[8];
+  {
+    float c[kTurns], s[kTurns];
+#pragma unroll
+    for (uint32_t i = 0; i < kTurns; ++i) {
+      double t = 0.0;
+      if (rotates) t = static_cast<double>(position) * static_cast<double>(a.inv_freq[8U * l + which * kTurns + i]) * 0.15915494309189533577;
+      t -= rint(t);  // turns, in [-1/2, 1/2]
+      sincospif(2.0F * static_cast<float>(t), &s[i], &c[i]);
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 8U; ++e) {
+      cosine[e] = __shfl_sync(0xffffffffU, c[e % kTurns], e / kTurns * kLanes + l);
+      sine[e] = __shfl_sync(0xffffffffU, s[e % kTurns], e / kTurns * kLanes + l);
+    }
+  }
+  uint8_t* layer = nullptr;
+  if (a.row_slot && sequence < a.cache.sequences && slot < kv_capacity(a.cache))
+    layer = kv_page(a.cache, sequence, slot / a.cache.page_tokens);
+  const uint32_t place = slot % a.cache.page_tokens;
+
+  for (uint32_t base = first; base < last; base += kStages * kHeadsPerWarp) {
+#pragma unroll
+    for (uint32_t stage = 0; stage < kStages; ++stage) {
+      const uint32_t head = base + stage * kHeadsPerWarp + which;
+      if (head - which >= last) break;
+      const bool live = l < kActive && head < last;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2U) : "memory");
+      float v0[8], v1[8];
+      {
+        uint4 raw[2U * kWords];
+#pragma unroll
+        for (uint32_t i = 0; i < 2U * kWords; ++i) raw[i] = live ? ring[stage][i][threadIdx.x] : make_uint4(0U, 0U, 0U, 0U);
+        load8(reinterpret_cast<const T*>(raw), v0);
+        load8(reinterpret_cast<const T*>(raw + kWords), v1);
+      }
+      fetch(head + (kStages - 1U) * kHeadsPerWarp, (stage + kStages - 1U) % kStages);
+      const bool is_value = head >= a.q_heads + kv;
+      float sum = 0.0F;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(v0[i], v0[i], fmaf(v1[i], v1[i], sum));
+      sum = head_sum<kLanes>(sum);
+      if (live && !is_value) {
+        const float* w = norm[head < a.q_heads ? 0 : 1];
+        const float r = rsqrtf(fmaf(sum, 1.0F / HD, a.eps));
+        float w0[8], w1[8];
+        load8(w + 8U * c0, w0);
+        load8(w + 8U * c1, w1);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float2 t = turn[8U * c0 + i];
-          const float low = v0[i], high = v1[i];
-          v0[i] = fmaf(low, t.x, -high * t.y);
-          v1[i] = fmaf(high, t.x, low * t.y);
+          v0[i] *= r * w0[i];
+          v1[i] *= r * w1[i];
+        }
+        if (rotates) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float low = v0[i], high = v1[i];
+            v0[i] = fmaf(low, cosine[i], -(high * sine[i]));
+            v1[i] = fmaf(high, cosine[i], low * sine[i]);
+          }
         }
       }
-    }
-    float scale = 0.0F;
-    __half stored = __float2half_rn(0.0F);
-    if (a.row_slot && a.cache.encoding != QLLM_KV_F16) {
-      float amax = 0.0F;
+      if (live && head < a.q_heads) {
+        T* q = static_cast<T*>(a.query) + static_cast<size_t>(row) * a.query_stride + static_cast<size_t>(head) * HD;
+        store8(q + 8U * c0, v0);
+        store8(q + 8U * c1, v1);
+      }
+      if (base + (stage + 1U) * kHeadsPerWarp <= a.q_heads) continue;
+      // ---- keys and values (whole warps from here on: the maximum of a record goes over lanes)
+      float scale = 0.0F;
+      __half stored = __float2half_rn(0.0F);
+      if (a.row_slot && a.cache.encoding != QLLM_KV_F16) {
+        float amax = 0.0F;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fmaxf(fabsf(v0[i]), fabsf(v1[i])));
-      scale = record_scale(head_max<kLanes>(amax), a.cache.encoding == QLLM_KV_Q4H ? 7.0F : 127.0F, &stored);
-    }
-    if (!live) continue;
-    if (head < a.q_heads) {
-      T* q = static_cast<T*>(a.query) + static_cast<size_t>(row) * a.query_stride + static_cast<size_t>(head) * HD;
-      store8(q + 8U * c0, v0);
-      store8(q + 8U * c1, v1);
-      continue;
-    }
-    const uint32_t h = head - a.q_heads - (is_value ? kv : 0U);
-    if (!is_value && a.key) {
-      T* k = static_cast<T*>(a.key) + static_cast<size_t>(row) * a.key_stride + static_cast<size_t>(h) * HD;
-      store8(k + 8U * c0, v0);
-      store8(k + 8U * c1, v1);
-    }
-    if (!layer) continue;
-    uint8_t* codes = layer + kv_codes_at(a.cache, is_value, place, h);
-    store_record8(a.cache, codes, c0, v0, scale);
-    store_record8(a.cache, codes, c1, v1, scale);
-    if (l == 0U) {
-      if (a.cache.encoding != QLLM_KV_F16)
-        *reinterpret_cast<__half*>(layer + kv_scale_at(a.cache, is_value, place, h)) = stored;
-      if (!is_value && a.slot_positions)
-        a.slot_positions[(static_cast<size_t>(sequence) * kv + h) * a.slot_stride + slot] = position;
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fmaxf(fabsf(v0[i]), fabsf(v1[i])));
+        scale = record_scale(head_max<kLanes>(amax), a.cache.encoding == QLLM_KV_Q4H ? 7.0F : 127.0F, &stored);
+      }
+      if (!live || head < a.q_heads) continue;
+      const uint32_t h = head - a.q_heads - (is_value ? kv : 0U);
+      if (!is_value && a.key) {
+        T* k = static_cast<T*>(a.key) + static_cast<size_t>(row) * a.key_stride + static_cast<size_t>(h) * HD;
+        store8(k + 8U * c0, v0);
+        store8(k + 8U * c1, v1);
+      }
+      if (!layer) continue;
+      uint8_t* codes = layer + kv_codes_at(a.cache, is_value, place, h);
+      store_record8(a.cache, codes, c0, v0, scale);
+      store_record8(a.cache, codes, c1, v1, scale);
+      if (l == 0U) {
+        if (a.cache.encoding != QLLM_KV_F16)
+          *reinterpret_cast<__half*>(layer + kv_scale_at(a.cache, is_value, place, h)) = stored;
+        if (!is_value && a.slot_positions)
+          a.slot_positions[(static_cast<size_t>(sequence) * kv + h) * a.slot_stride + slot] = position;
+      }
     }
   }
 }
 
 template <typename T, int HD>
 int launch(const NormRopeStoreArgs& a, cudaStream_t stream) {
+  constexpr uint32_t kHeadsPerWarp = HD == 64 ? 8U : HD == 128 ? 4U : 2U;
   const uint32_t heads = a.q_heads + (a.row_slot ? 2U : 1U) * a.cache.kv_heads;
-  norm_rope_store_kernel<T, HD><<<dim3(a.rows), kThreads, 0, stream>>>(a, heads);
+  const uint32_t all = (heads + kHeadsPerWarp - 1U) / kHeadsPerWarp;
+  // as many passes to a warp as leave kWarpsWanted of them
+  const uint32_t passes = static_cast<uint32_t>(max(static_cast<uint64_t>(1U), min(static_cast<uint64_t>(all), static_cast<uint64_t>(all) * a.rows / kWarpsWanted)));
+  const uint32_t tasks = (all + passes - 1U) / passes;
+  const uint64_t blocks = (static_cast<uint64_t>(tasks) * a.rows + kThreads / 32U - 1U) / (kThreads / 32U);
+  if (blocks > 0x7FFFFFFFULL) return fail(QLLM_INVALID_ARGUMENT, "QK norm / RoPE / KV store: too many rows");
   count_launch();
-  return check_launch("qk_norm_rope_store");
+  return check_cuda(launch_ordered(norm_rope_store_kernel<T, HD>, dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, stream, a, tasks, passes),
+                    "qk_norm_rope_store");
 }
 
 template <typename T>
