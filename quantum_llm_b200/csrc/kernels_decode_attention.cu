@@ -43,7 +43,7 @@ constexpr uint32_t kWarps = 4;
 constexpr uint32_t kThreads = 32 * kWarps;
 constexpr uint32_t kUnit = 64;          // tokens
 constexpr uint32_t kItemBytes = 96U * 1024U;  // what a block could read in the time an item costs it beside its tokens
-constexpr uint32_t kMaxBlocks = 512;    // of the first launch; places in the workspace
+constexpr uint32_t kMaxBlocks = 768;    // of the first launch; places in the workspace
 constexpr uint32_t kHeads = 8;          // query heads of an item per kv head
 constexpr uint32_t kWeightTokens = 4 * kThreads;
 // log2: the largest p of a warp stands between 2^kLift (when the reference was set) and 2^kTop < 65504
@@ -167,8 +167,9 @@ template <int ENC, int HD>
 struct Layout {
   static constexpr bool kStaged = ENC == QLLM_KV_Q8;
   // blocks of 16 keys that a warp takes at a time: 16 - 64 registers of K and of V (Q4H, HD 128: 4 blocks spill, 31 us
-  // against 25 us with 2 for one sequence of 32768)
-  static constexpr int kBlocks = ENC == QLLM_KV_F16 ? (HD == 64 ? 2 : 1) : ENC == QLLM_KV_Q4H ? (HD == 64 ? 4 : 2) : 1;
+  // against 25 us with 2 for one sequence of 32768; F16, HD 64: 2 blocks leave room for three blocks of threads to a
+  // multiprocessor instead of four, 64 us against 57 us for 7 sequences of up to 20001)
+  static constexpr int kBlocks = ENC == QLLM_KV_Q4H ? 2 : 1;
   static constexpr int kRegs = ENC == QLLM_KV_F16 ? HD / 4 : ENC == QLLM_KV_Q4H ? HD / 16 : 1;  // of K, and of V, per block
   static constexpr int kKWords = ENC == QLLM_KV_Q4H ? (HD % 128 == 0 ? 4 : 2) : 4;      // words per load
   static constexpr int kVWords = ENC == QLLM_KV_Q4H ? (HD == 128 ? 2 : HD == 256 ? 4 : 1) : 4;
@@ -228,7 +229,7 @@ struct Traits {
   static constexpr int kTerms = kPrecise ? 2 : 1;
   static constexpr int kSteps = HD / 16;
   static constexpr bool kQueryInRegisters = HD <= 128;
-  static constexpr int kBlocksPerSm = HD <= 128 ? 3 : 2;
+  static constexpr int kBlocksPerSm = HD == 64 ? 4 : HD == 128 ? 3 : 2;
   // the queries of one kv head: rows 16 bytes apart from a multiple of 128 (free of bank conflicts), then fragments in their place
   static constexpr int kQueryPitch = HD * static_cast<int>(sizeof(T)) + 16;
   static constexpr size_t kQueryBytes = static_cast<size_t>(kHeads) * kQueryPitch;
@@ -988,26 +989,33 @@ __device__ __forceinline__ void add_weights(const DecodeAttentionArgs& a, const 
       if (lane == 0U) lse[g] = value;
     }
     __syncthreads();
-    const float* scores = plan.scores + (static_cast<size_t>(s) * a.q_heads + head0) * capacity;
+    const float* scores = plan.scores + (static_cast<size_t>(s) * a.q_heads + head0) * capacity + threadIdx.x;
     const float* start = g0 ? a.weights_out : a.weights_in;
     for (uint32_t t0 = chunk * kWeightTokens; t0 < n; t0 += chunks * kWeightTokens) {
-      float before[kEach], score[kHeads][kEach];
+      const uint32_t left = n - t0;  // tokens from here on
+      float added[kEach], score[kHeads][kEach];
 #pragma unroll
-      for (uint32_t i = 0; i < kEach; ++i) {
-        const uint32_t t = t0 + i * kThreads + threadIdx.x;
-        before[i] = start && t < n ? start[row + t] : 0.0F;
+      for (uint32_t g = 0; g < kHeads; ++g) {
+        if (g >= here) break;
+        const float* from = scores + static_cast<size_t>(g) * capacity + t0;
 #pragma unroll
-        for (uint32_t g = 0; g < kHeads; ++g) score[g][i] = g < here && t < n ? scores[static_cast<size_t>(g) * capacity + t] : -INFINITY;
+        for (uint32_t i = 0; i < kEach; ++i) score[g][i] = i * kThreads + threadIdx.x < left ? from[i * kThreads] : 0.0F;
       }
 #pragma unroll
-      for (uint32_t i = 0; i < kEach; ++i) {
-        const uint32_t t = t0 + i * kThreads + threadIdx.x;
-        float added = 0.0F;
+      for (uint32_t i = 0; i < kEach; ++i)
+        added[i] = start && i * kThreads + threadIdx.x < left ? start[row + t0 + i * kThreads + threadIdx.x] : 0.0F;
+      float sum[kEach] = {};
 #pragma unroll
-        for (uint32_t g = 0; g < kHeads; ++g)
-          if (g < here) added += exp2_fast(score[g][i] - lse[g]);
-        if (t < n) a.weights_out[row + t] = before[i] + added;
+      for (uint32_t g = 0; g < kHeads; ++g) {
+        if (g >= here) break;
+        const float of = lse[g];
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) sum[i] += exp2_fast(score[g][i] - of);
       }
+      float* to = a.weights_out + row + t0 + threadIdx.x;
+#pragma unroll
+      for (uint32_t i = 0; i < kEach; ++i)
+        if (i * kThreads + threadIdx.x < left) to[i * kThreads] = added[i] + sum[i];
     }
   }
 }

@@ -32,7 +32,8 @@ constexpr uint32_t kMaxCluster = 8;
 constexpr uint32_t kAhead = 8;
 constexpr uint32_t kMaxKeys = 48U * 1024U;  // of one block in shared memory; longer rows read weights and positions again
 constexpr uint32_t kMoveThreads = 256;
-constexpr uint32_t kMoveBatch = 64;       // moves
+constexpr uint32_t kMoveBatch = 64;       // moves (32: 142 us, 64: 135 us, 128: 136 us for 8 x 8 rows of 8455)
+constexpr uint32_t kMoveBlocks = 5;       // per multiprocessor, all of them at once
 
 // Workspace: [rows] headers, then [rows][most] pairs {freed slot, kept slot}.
 struct RowHeader {
@@ -62,15 +63,15 @@ struct Counts {
 
 __global__ void __launch_bounds__(kSelectThreads, 2)
 kv_select_kernel(const __grid_constant__ KvEvictArgs a, RowHeader* headers, uint2* pairs, uint32_t most, uint32_t keys_held) {
-  extern __shared__ uint32_t keys[];
+  extern __shared__ __align__(16) uint32_t keys[];
   __shared__ alignas(16) uint32_t bins[2][kBins];
-  __shared__ uint32_t warp_sums[kSelectWarps], chosen[3];
+  __shared__ uint32_t warp_sums[kSelectWarps], chosen[4];
   __shared__ Counts warp_counts[kSelectWarps], counts;
   const cg::cluster_group cluster = cg::this_cluster();
   const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank();
   const size_t row = blockIdx.x / blocks;
   const uint32_t s = static_cast<uint32_t>(row / a.cache.kv_heads);
-  const uint32_t tid = threadIdx.x, lane = tid & 31U, warp = tid >> 5U, below = (1U << lane) - 1U;
+  const uint32_t tid = threadIdx.x, lane = tid & 31U, warp = tid >> 5U;
   const uint32_t n = min(a.lengths_in[s], kv_capacity(a.cache));
   const uint32_t m = min(n, a.budget);
   const uint32_t next = a.next_positions[s];
@@ -78,14 +79,35 @@ kv_select_kernel(const __grid_constant__ KvEvictArgs a, RowHeader* headers, uint
   const uint32_t* pos = a.positions_in + row * a.stride;
   float* w_out = a.weights_out + row * a.stride;
   uint32_t* pos_out = a.positions_out + row * a.stride;
-  // this block's slots [first, first + count)
-  const uint32_t slice = ((n + blocks - 1U) / blocks + 31U) & ~31U;
-  const uint32_t first = min(n, rank * slice), count = min(slice, n - first);
-  if (n == m) {  // everything stays; the whole cluster leaves
-    for (uint32_t t = first + tid; t < first + count; t += kSelectThreads) {
-      if (w_out != w) w_out[t] = w[t];
-      if (pos_out != pos) pos_out[t] = pos[t];
+  // this block's slots [first, first + count), in quads: a thread takes four neighbours at a time
+  const uint32_t slice = ((n + blocks - 1U) / blocks + 127U) & ~127U;
+  const uint32_t first = min(n, rank * slice), count = min(slice, n - first), quads = (count + 3U) / 4U;
+  const bool held = slice <= keys_held;
+  bool crowded = false;
+  // The keys, kAhead loads of a thread in flight.  Where the outputs are other arrays, they get what would be there
+  // without a move: the slots below m as they are, zero weights behind.
+  const auto make_keys = [&] {
+    for (uint32_t j = tid; j < count; j += kAhead * kSelectThreads) {
+      float weight[kAhead];
+      uint32_t position[kAhead];
+#pragma unroll
+      for (uint32_t u = 0; u < kAhead; ++u) {
+        const uint32_t i = j + u * kSelectThreads;
+        weight[u] = i < count ? w[first + i] : 0.0F;
+        position[u] = i < count ? pos[first + i] : 0U;
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < kAhead; ++u) {
+        const uint32_t i = j + u * kSelectThreads, t = first + i;
+        if (i >= count) continue;
+        if (held && n > m) keys[i] = keep_key(a, weight[u], position[u], next, crowded);
+        if (w_out != w) w_out[t] = t < m ? weight[u] : 0.0F;
+        if (pos_out != pos && t < m) pos_out[t] = position[u];
+      }
     }
+  };
+  make_keys();
+  if (n == m) {  // everything stays; the whole cluster leaves
     if (rank == 0U && tid == 0U) headers[row] = {n, m, 0U, 0U};
     return;
   }
@@ -93,60 +115,51 @@ kv_select_kernel(const __grid_constant__ KvEvictArgs a, RowHeader* headers, uint
     if (blocks == 1U) __syncthreads();
     else cluster.sync();
   };
-  const bool held = slice <= keys_held;
-  bool crowded = false;
-  const auto make_key = [&](uint32_t i) { return keep_key(a, w[first + i], pos[first + i], next, crowded); };
-  const auto key_of = [&](uint32_t i) { return held ? keys[i] : make_key(i); };
-
-  // the keys, kAhead loads of a thread in flight
-  const uint32_t rounds = (count + kSelectThreads - 1U) / kSelectThreads;
-  const auto make_keys = [&] {
-    if (!held) return;
-    for (uint32_t j = 0; j < rounds; j += kAhead) {
-      float weight[kAhead];
-      uint32_t position[kAhead];
+  const auto four_keys = [&](uint32_t quad, uint32_t (&key)[4]) {
+    if (held) {
+      const uint4 v = reinterpret_cast<const uint4*>(keys)[quad];
+      key[0] = v.x;
+      key[1] = v.y;
+      key[2] = v.z;
+      key[3] = v.w;
+    } else {
 #pragma unroll
-      for (uint32_t u = 0; u < kAhead; ++u) {
-        const uint32_t i = (j + u) * kSelectThreads + tid;
-        weight[u] = i < count ? w[first + i] : 0.0F;
-        position[u] = i < count ? pos[first + i] : 0U;
-      }
-#pragma unroll
-      for (uint32_t u = 0; u < kAhead; ++u) {
-        const uint32_t i = (j + u) * kSelectThreads + tid;
-        if (i < count) keys[i] = keep_key(a, weight[u], position[u], next, crowded);
+      for (uint32_t u = 0; u < 4U; ++u) {
+        const uint32_t i = 4U * quad + u;
+        key[u] = i < count ? keep_key(a, w[first + i], pos[first + i], next, crowded) : 0U;
       }
     }
   };
 
   // ---- the m-th largest key
+  uint32_t threshold = 0U, ties = 0U;  // kept: keys above the threshold, and the first `ties` slots of that key
   uint32_t left = m, prefix = 0U, shift = 21U, buffer = 0U;
   for (uint32_t i = tid; i < kBins; i += kSelectThreads) bins[0][i] = 0U;
-  make_keys();
   __syncthreads();
+  const uint32_t rounds = (quads + kSelectThreads - 1U) / kSelectThreads;
   for (;;) {
     const uint32_t top = shift + (shift == 0U ? 10U : 11U);  // bits from here on are the prefix
-    for (uint32_t j = 0; j < rounds; j += 4U) {
-      uint32_t four[4];
-#pragma unroll
-      for (uint32_t u = 0; u < 4U; ++u) {
-        const uint32_t i = (j + u) * kSelectThreads + tid;
-        four[u] = i < count ? key_of(i) : 0U;
-      }
+    for (uint32_t j = 0; j < rounds; ++j) {
+      const uint32_t quad = j * kSelectThreads + tid;
+      uint32_t four[4] = {0U, 0U, 0U, 0U};
+      if (quad < quads) four_keys(quad, four);
 #pragma unroll
       for (uint32_t u = 0; u < 4U; ++u) {
         const uint32_t key = four[u];
-        const bool counts_here = (j + u) * kSelectThreads + tid < count && (shift == 21U || (key >> top) == prefix);
-        // the digit of the warp's first counting lane is added once for all lanes that share it: equal weights would
-        // otherwise queue up at one address
+        const bool counts_here = 4U * quad + u < count && (shift == 21U || (key >> top) == prefix);
         const uint32_t who = __ballot_sync(0xffffffffU, counts_here);
-        if (who == 0U) continue;
         const uint32_t digit = (key >> shift) & (shift == 0U ? 1023U : 2047U);
-        const uint32_t leader = __ffs(who) - 1U;
-        const uint32_t common = __shfl_sync(0xffffffffU, digit, leader);
-        const uint32_t same = __ballot_sync(0xffffffffU, counts_here && digit == common);
-        if (lane == leader) atomicAdd(&bins[buffer][common], static_cast<uint32_t>(__popc(same)));
-        else if (counts_here && digit != common) atomicAdd(&bins[buffer][digit], 1U);
+        if (__popc(who) >= 8) {
+          // the digit of the warp's first counting lane is added once for all lanes that share it: equal weights would
+          // otherwise queue up at one address
+          const uint32_t leader = __ffs(who) - 1U;
+          const uint32_t common = __shfl_sync(0xffffffffU, digit, leader);
+          const uint32_t same = __ballot_sync(0xffffffffU, counts_here && digit == common);
+          if (lane == leader) atomicAdd(&bins[buffer][common], static_cast<uint32_t>(__popc(same)));
+          else if (counts_here && digit != common) atomicAdd(&bins[buffer][digit], 1U);
+        } else if (counts_here) {
+          atomicAdd(&bins[buffer][digit], 1U);
+        }
       }
     }
     barrier();
@@ -185,6 +198,7 @@ kv_select_kernel(const __grid_constant__ KvEvictArgs a, RowHeader* headers, uint
       }
       chosen[0] = bin - k;
       chosen[1] = before;
+      chosen[3] = v[0];
     }
     if (tid == 0U) chosen[2] = last_bin;
     __syncthreads();
@@ -198,27 +212,42 @@ kv_select_kernel(const __grid_constant__ KvEvictArgs a, RowHeader* headers, uint
     }
     prefix = (prefix << (shift == 0U ? 10U : 11U)) | chosen[0];
     left -= chosen[1];
-    if (shift == 0U) break;
+    if (left == chosen[3] && prefix != 0U) {  // the cut falls between two bins: every key of this one is kept (a cache that
+      threshold = (prefix << shift) - 1U;     // evicts a slot a step is done after one digit most of the time)
+      break;
+    }
+    if (shift == 0U) {
+      threshold = prefix;
+      ties = left;
+      break;
+    }
     shift = shift == 21U ? 10U : 0U;
     __syncthreads();  // `chosen` has been read
   }
-  const uint32_t threshold = prefix, ties = left;  // the first `ties` slots of that key are kept
 
-  // ---- ranks.  Each warp walks a contiguous segment of the block's slots.
-  const uint32_t segment = ((count + kSelectWarps - 1U) / kSelectWarps + 31U) & ~31U;
-  const uint32_t seg0 = min(count, warp * segment), seg1 = min(count, seg0 + segment);
+  // ---- ranks.  Each warp walks a contiguous segment of the block's quads.
+  const uint32_t segment = ((quads + kSelectWarps - 1U) / kSelectWarps + 31U) & ~31U;
+  const uint32_t seg0 = min(quads, warp * segment), seg1 = min(quads, seg0 + segment);
   Counts mine{};
-  for (uint32_t i0 = seg0; i0 < seg1; i0 += 32U) {
-    const uint32_t i = i0 + lane;
-    const uint32_t key = i < seg1 ? key_of(i) : 0U;
-    const uint32_t over = __ballot_sync(0xffffffffU, i < seg1 && key > threshold);
-    const uint32_t tied = __ballot_sync(0xffffffffU, i < seg1 && key == threshold);
-    // lanes whose slot lies below m
-    const uint32_t under = first + i0 >= m ? 0U : m - first - i0 >= 32U ? 0xffffffffU : (1U << (m - first - i0)) - 1U;
-    mine.over[0] += __popc(over & under);
-    mine.over[1] += __popc(over & ~under);
-    mine.tied[0] += __popc(tied & under);
-    mine.tied[1] += __popc(tied & ~under);
+  for (uint32_t q0 = seg0; q0 < seg1; q0 += 32U) {
+    const uint32_t quad = q0 + lane;
+    if (quad >= seg1) continue;
+    uint32_t key[4];
+    four_keys(quad, key);
+#pragma unroll
+    for (uint32_t u = 0; u < 4U; ++u) {
+      const uint32_t i = 4U * quad + u, side = first + i < m ? 0U : 1U;
+      const uint32_t over = i < count && key[u] > threshold ? 1U : 0U, tied = i < count && key[u] == threshold ? 1U : 0U;
+      mine.over[0] += side ? 0U : over;
+      mine.over[1] += side ? over : 0U;
+      mine.tied[0] += side ? 0U : tied;
+      mine.tied[1] += side ? tied : 0U;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    mine.over[k] = __reduce_add_sync(0xffffffffU, mine.over[k]);
+    mine.tied[k] = __reduce_add_sync(0xffffffffU, mine.tied[k]);
   }
   if (lane == 0U) warp_counts[warp] = mine;
   __syncthreads();
@@ -234,56 +263,86 @@ kv_select_kernel(const __grid_constant__ KvEvictArgs a, RowHeader* headers, uint
       all.tied[k] = __reduce_add_sync(0xffffffffU, v.tied[k]);
     }
   }
-  if (tid == 0U) counts = all;
-  if (blocks > 1U) cluster.sync();
   // ties, kept slots below m and movers in the blocks before this one
   uint32_t ties_before = 0U, kept_before = 0U, movers_before = 0U;
-  for (uint32_t b = 0; b < rank; ++b) {
-    const Counts v = *cluster.map_shared_rank(&counts, b);
-    const uint32_t kept_ties = min(v.tied[0], ties - min(ties, ties_before));
-    kept_before += v.over[0] + kept_ties;
-    movers_before += v.over[1] + min(v.tied[1], ties - min(ties, ties_before + v.tied[0]));
-    ties_before += v.tied[0] + v.tied[1];
+  if (blocks > 1U) {
+    if (tid == 0U) counts = all;
+    cluster.sync();
+    for (uint32_t b = 0; b < rank; ++b) {
+      const Counts v = *cluster.map_shared_rank(&counts, b);
+      kept_before += v.over[0] + min(v.tied[0], ties - min(ties, ties_before));
+      movers_before += v.over[1] + min(v.tied[1], ties - min(ties, ties_before + v.tied[0]));
+      ties_before += v.tied[0] + v.tied[1];
+    }
+    cluster.sync();  // nobody leaves while its counts are read
   }
-  if (blocks > 1U) cluster.sync();  // nobody leaves while its counts are read
   // ... and in the warps before this one (a segment's ties all come after those of the segments before it)
-  const uint32_t kept_ties = min(before.tied[0], ties - min(ties, ties_before));
-  uint32_t kept = kept_before + before.over[0] + kept_ties;
+  const uint32_t kept = kept_before + before.over[0] + min(before.tied[0], ties - min(ties, ties_before));
   uint32_t movers = movers_before + before.over[1] + min(before.tied[1], ties - min(ties, ties_before + before.tied[0]));
   uint32_t tied_so_far = ties_before + before.tied[0] + before.tied[1];
-  uint32_t holes = min(m, first + seg0) - kept;
+  uint32_t holes = min(m, first + 4U * seg0) - kept;
   uint2* list = pairs + row * most;
-  for (uint32_t i4 = seg0; i4 < seg1; i4 += 32U * kAhead) {
-    // what stays below m is copied where the outputs are other arrays than the inputs
-    float weight[kAhead];
-    uint32_t position[kAhead];
+  for (uint32_t q0 = seg0; q0 < seg1; q0 += 32U) {
+    const uint32_t quad = q0 + lane;
+    uint32_t key[4] = {0U, 0U, 0U, 0U};
+    if (quad < seg1) four_keys(quad, key);
+    uint32_t tied = 0U, inside = 0U;  // bit u: the lane's slot u counts
 #pragma unroll
-    for (uint32_t u = 0; u < kAhead; ++u) {
-      const uint32_t i = i4 + 32U * u + lane, t = first + i;
-      weight[u] = w_out != w && i < seg1 && t < m ? w[t] : 0.0F;
-      position[u] = pos_out != pos && i < seg1 && t < m ? pos[t] : 0U;
+    for (uint32_t u = 0; u < 4U; ++u) {
+      if (quad < seg1 && 4U * quad + u < count) inside |= 1U << u;
+      if (key[u] == threshold) tied |= 1U << u;
     }
+    tied &= inside;
+    uint32_t tie = tied_so_far;  // rank of the lane's first tie
+    if (__any_sync(0xffffffffU, tied != 0U)) {
+      uint32_t upto = __popc(tied);
 #pragma unroll
-    for (uint32_t u = 0; u < kAhead; ++u) {
-      const uint32_t i = i4 + 32U * u + lane, t = first + i;
-      const bool here = i < seg1;
-      const uint32_t key = here ? key_of(i) : 0U;
-      const uint32_t tied = __ballot_sync(0xffffffffU, here && key == threshold);
-      const bool keep = here && (key > threshold || (key == threshold && tied_so_far + __popc(tied & below) < ties));
-      tied_so_far += __popc(tied);
-      const bool hole = here && t < m && !keep, mover = here && t >= m && keep;
-      const uint32_t hole_mask = __ballot_sync(0xffffffffU, hole), mover_mask = __ballot_sync(0xffffffffU, mover);
-      const uint32_t hole_rank = holes + __popc(hole_mask & below), mover_rank = movers + __popc(mover_mask & below);
-      if (hole && hole_rank < most) list[hole_rank].x = t;
-      if (mover && mover_rank < most) list[mover_rank].y = t;
-      holes += __popc(hole_mask);
-      movers += __popc(mover_mask);
-      if (here && t < m && keep) {
-        if (w_out != w) w_out[t] = weight[u];
-        if (pos_out != pos) pos_out[t] = position[u];
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffU, upto, o);
+        if (lane >= static_cast<uint32_t>(o)) upto += t;
       }
-      if (here && t >= m && !keep) w_out[t] = 0.0F;
+      tie += upto - __popc(tied);
+      tied_so_far += __shfl_sync(0xffffffffU, upto, 31);
     }
+    uint32_t hole = 0U, mover = 0U;
+#pragma unroll
+    for (uint32_t u = 0; u < 4U; ++u) {
+      const uint32_t t = first + 4U * quad + u;
+      const bool keep = key[u] > threshold || ((tied >> u & 1U) && tie < ties);
+      tie += tied >> u & 1U;
+      if (!(inside >> u & 1U)) continue;
+      if (t < m) {
+        if (!keep) hole |= 1U << u;
+      } else if (keep) {
+        mover |= 1U << u;
+      } else if (w_out == w) {
+        w_out[t] = 0.0F;
+      }
+    }
+    if (!__any_sync(0xffffffffU, (hole | mover) != 0U)) continue;
+    const uint32_t both = __popc(hole) | __popc(mover) << 16U;  // at most 128 of each
+    uint32_t upto = both;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t t = __shfl_up_sync(0xffffffffU, upto, o);
+      if (lane >= static_cast<uint32_t>(o)) upto += t;
+    }
+    uint32_t hole_rank = holes + ((upto - both) & 0xffffU), mover_rank = movers + ((upto - both) >> 16U);
+#pragma unroll
+    for (uint32_t u = 0; u < 4U; ++u) {
+      const uint32_t t = first + 4U * quad + u;
+      if (hole >> u & 1U) {
+        if (hole_rank < most) list[hole_rank].x = t;
+        ++hole_rank;
+      }
+      if (mover >> u & 1U) {
+        if (mover_rank < most) list[mover_rank].y = t;
+        ++mover_rank;
+      }
+    }
+    const uint32_t all_lanes = __shfl_sync(0xffffffffU, upto, 31);
+    holes += all_lanes & 0xffffU;
+    movers += all_lanes >> 16U;
   }
   // the last warp of the last block has counted every mover
   if (rank == blocks - 1U && warp == kSelectWarps - 1U && lane == 0U) headers[row] = {n, m, min(movers, most), 0U};
@@ -295,18 +354,58 @@ __host__ __device__ __forceinline__ uint32_t record_words(uint32_t encoding, uin
   return 2U * (encoding == QLLM_KV_F16 ? hd / 8U : encoding == QLLM_KV_Q4H ? hd / 32U + 1U : hd / 4U + 1U);
 }
 
-// grid (rows, chunks).  Moves in batches: first a thread per move finds its two pages and moves weight and position, then
-// all threads copy words, kAtOnce of them in flight each.
+// Moves in batches: first a thread per move finds its two pages and moves weight and position, then all threads copy
+// words, kAtOnce of them in flight each.  The batches of all rows stand in one line, of which each block takes an equal
+// share: rows that move nothing cost no blocks (empty ones took 8 us of 32 for 192 rows).
 template <uint32_t ENC>
 __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_constant__ KvEvictArgs a, const RowHeader* headers,
                                                                const uint2* pairs, uint32_t most) {
   constexpr int kAtOnce = 4;
   __shared__ uint8_t* codes[2][kMoveBatch];   // K codes of target and source, null: no page
   __shared__ uint8_t* scales[2][ENC == QLLM_KV_Q4H ? kMoveBatch : 1];
+  __shared__ unsigned long long warp_batches[kMoveThreads / 32U], start_base;
+  __shared__ uint32_t start_row;
+  const uint32_t kv = a.cache.kv_heads, rows = a.cache.sequences * kv, lane = threadIdx.x & 31U, warp = threadIdx.x >> 5U;
   pdl_wait();
-  const uint32_t row = blockIdx.x, s = row / a.cache.kv_heads, h = row % a.cache.kv_heads;
-  const RowHeader header = headers[row];
-  if (h == 0U && blockIdx.y == 0U && threadIdx.x == 0U) a.lengths_out[s] = header.kept;
+  for (uint32_t s = blockIdx.x * kMoveThreads + threadIdx.x; s < a.cache.sequences; s += gridDim.x * kMoveThreads)
+    a.lengths_out[s] = headers[static_cast<size_t>(s) * kv].kept;
+  // ---- this block's share of the batches
+  const auto batches_of = [&](uint32_t row) { return (headers[row].moves + kMoveBatch - 1U) / kMoveBatch; };
+  const uint32_t per_thread = (rows + kMoveThreads - 1U) / kMoveThreads;
+  const uint32_t r0 = min(rows, threadIdx.x * per_thread), r1 = min(rows, r0 + per_thread);
+  unsigned long long own = 0ULL;
+  for (uint32_t r = r0; r < r1; ++r) own += batches_of(r);
+  unsigned long long upto = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long t = __shfl_up_sync(0xffffffffU, upto, o);
+    if (lane >= static_cast<uint32_t>(o)) upto += t;
+  }
+  if (lane == 31U) warp_batches[warp] = upto;
+  __syncthreads();
+  unsigned long long total = 0ULL, before = upto - own;
+#pragma unroll
+  for (uint32_t w = 0; w < kMoveThreads / 32U; ++w) {
+    if (w < warp) before += warp_batches[w];
+    total += warp_batches[w];
+  }
+  unsigned long long batch = blockIdx.x * total / gridDim.x;
+  const unsigned long long end = (blockIdx.x + 1ULL) * total / gridDim.x;
+  if (batch == end) return;
+  if (before <= batch && batch < before + own) {
+    uint32_t r = r0;
+    unsigned long long base = before;
+    for (;; ++r) {
+      const uint32_t n = batches_of(r);
+      if (batch < base + n) break;
+      base += n;
+    }
+    start_row = r;
+    start_base = base;
+  }
+  __syncthreads();
+  uint32_t row = start_row;
+  unsigned long long base = start_base;
   const uint32_t pt = a.cache.page_tokens, hd = a.cache.head_dim;
   const uint32_t words = record_words(ENC, hd), at_once = kMoveThreads / words;  // moves of a block side by side
   const uint32_t local = threadIdx.x / words, part = threadIdx.x % words;
@@ -316,10 +415,16 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_cons
   // from a record's K codes (scale) to the thread's word
   const size_t to_value = value ? kv_codes_at(a.cache, true, 0U, 0U) : 0U;
   const size_t delta = to_value + (ENC == QLLM_KV_Q8 || is_scale ? 0U : 16U * word);
-  const uint2* list = pairs + static_cast<size_t>(row) * most;
-  const size_t at = static_cast<size_t>(row) * a.stride;
-  for (uint32_t i0 = blockIdx.y * kMoveBatch; i0 < header.moves; i0 += gridDim.y * kMoveBatch) {
-    const uint32_t count = min(kMoveBatch, header.moves - i0);
+  for (; batch < end; ++batch) {
+    uint32_t moves = headers[row].moves;
+    while (batch - base >= (moves + kMoveBatch - 1U) / kMoveBatch) {
+      base += (moves + kMoveBatch - 1U) / kMoveBatch;
+      moves = headers[++row].moves;
+    }
+    const uint32_t i0 = static_cast<uint32_t>(batch - base) * kMoveBatch;
+    const uint32_t count = min(kMoveBatch, moves - i0), s = row / kv, h = row % kv;
+    const uint2* list = pairs + static_cast<size_t>(row) * most;
+    const size_t at = static_cast<size_t>(row) * a.stride;
     __syncthreads();  // the batch before has been copied
     if (threadIdx.x < 2U * kMoveBatch) {
       const uint32_t i = threadIdx.x % kMoveBatch, side = threadIdx.x / kMoveBatch;
@@ -405,7 +510,7 @@ int launch_kv_evict(const KvEvictArgs& a, cudaStream_t stream) {
   while (cluster < kMaxCluster && ((rows * cluster < static_cast<uint32_t>(sms) && capacity / cluster > kSlotsPerBlock) ||
                                    capacity / cluster > kMaxKeys))
     cluster *= 2U;
-  const uint32_t slice = ((capacity + cluster - 1U) / cluster + 31U) & ~31U;
+  const uint32_t slice = ((capacity + cluster - 1U) / cluster + 127U) & ~127U;
   const uint32_t keys_held = min(slice, kMaxKeys);
   e = cudaFuncSetAttribute(kv_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * sizeof(uint32_t));
   if (e != cudaSuccess) return check_cuda(e, "kv_evict shared memory opt-in");
@@ -425,12 +530,9 @@ int launch_kv_evict(const KvEvictArgs& a, cudaStream_t stream) {
   const int rc = check_cuda(cudaLaunchKernelEx(&config, kv_select_kernel, a, headers, pairs, most, keys_held), "kv_evict selection");
   if (rc) return rc;
 
-  // a block per batch, up to 32 blocks per multiprocessor (8: 143 us, 32: 133 us, 64: 133 us for 8 x 8 rows of 8455 moves: rows
-  // that move less leave room to the others)
-  const uint32_t wanted = (most + kMoveBatch - 1U) / kMoveBatch, room = 32U * static_cast<uint32_t>(sms) / rows;
-  const uint32_t chunks = max(1U, min(wanted, room));
+  const uint64_t batches = static_cast<uint64_t>(rows) * ((most + kMoveBatch - 1U) / kMoveBatch);
+  const dim3 grid(static_cast<uint32_t>(max(static_cast<uint64_t>(1U), min(batches, static_cast<uint64_t>(kMoveBlocks) * sms)))), block(kMoveThreads);
   count_launch();
-  const dim3 grid(rows, chunks), block(kMoveThreads);
   if (a.cache.encoding == QLLM_KV_F16) e = launch_pdl(kv_move_kernel<QLLM_KV_F16>, grid, block, 0, stream, a, headers, pairs, most);
   else if (a.cache.encoding == QLLM_KV_Q4H) e = launch_pdl(kv_move_kernel<QLLM_KV_Q4H>, grid, block, 0, stream, a, headers, pairs, most);
   else e = launch_pdl(kv_move_kernel<QLLM_KV_Q8>, grid, block, 0, stream, a, headers, pairs, most);

@@ -7,7 +7,7 @@
 //
 // Everything between the load of a value and its one rounding to the row's type (or to the record)
 // is FP32.  The angle is reduced in FP64: position * inv_freq as an FP32 product is off by up to
-// 2^-24 of an angle of thousands of turns, i.e. by whole tenths of a turn at position 10^6.
+// 2^-24 of the angle, i.e. by a hundredth of a turn at position 10^6.
 //
 // HBM-bound: a row is read once and its results written once.  A lane owns the eight values at i and
 // the eight at i + R/2 (the pair that a rotation mixes), so a head of 128 is eight lanes with two
