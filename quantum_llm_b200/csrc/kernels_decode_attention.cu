@@ -1021,7 +1021,7 @@ __device__ __forceinline__ void add_weights(const DecodeAttentionArgs& a, const 
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_constant__ DecodeAttentionArgs a, const __grid_constant__ Plan plan,
+__global__ void __launch_bounds__(kThreads, 8) decode_join_kernel(const __grid_constant__ DecodeAttentionArgs a, const __grid_constant__ Plan plan,
                                                                uint32_t joins, uint32_t ways, uint32_t chunks) {
   pdl_wait();
   const uint32_t warp = threadIdx.x >> 5U, first_join = gridDim.x - joins;
