@@ -110,6 +110,11 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
@@ -146,6 +151,25 @@ __device__ __forceinline__ void load_words(uint32_t* d, const uint8_t* p) {
     asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(d[0]) : "l"(p));
 }
 
+// Shared memory by its 32-bit address, the offset in the instruction.
+template <int kOffset>
+__device__ __forceinline__ uint32_t shared_word(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(v) : "r"(at), "n"(kOffset) : "memory");
+  return v;
+}
+template <int kOffset>
+__device__ __forceinline__ float shared_half(uint32_t at) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1+%2];" : "=h"(v) : "r"(at), "n"(kOffset) : "memory");
+  return __half2float(__ushort_as_half(v));
+}
+template <int kStep, int kN, int kI = 0>
+__device__ __forceinline__ void shared_words(uint32_t at, uint32_t (&w)[kN]) {
+  w[kI] = shared_word<kStep * kI>(at);
+  if constexpr (kI + 1 < kN) shared_words<kStep, kN, kI + 1>(at, w);
+}
+
 // Four nibbles (two's complement) at bits 0, 4, 8, 12 of each 16-bit half -> pairs of F16, one per nibble position:
 // 0x6400 | (n ^ 8) is 1024 + n + 8, and with the nibble four bits higher 1024 + 16 (n + 8).
 __device__ __forceinline__ void nibbles_to_half(uint32_t w, uint32_t (&h)[4]) {
@@ -179,20 +203,26 @@ struct Layout {
   static constexpr int kStage = 2 * 16 * kPitch;
   static constexpr int kStages = HD == 64 ? 4 : HD <= 192 ? 3 : 2;  // as many as leave room for kBlocksPerSm
 
-  // dimensions of half-words 0 and 1 of fragment register b (0, 1) in k step `ks`, lane c
-  static __device__ __forceinline__ uint32_t query_dim(int ks, int b, int half, uint32_t c) {
-    if constexpr (ENC == QLLM_KV_F16) return 8U * (c + 4U * (ks / 2)) + 4U * (ks % 2) + 2U * b + half;
-    if constexpr (ENC == QLLM_KV_Q8) return 2U * (c + 4U * (2 * ks + b)) + half;
-    const uint32_t word = (c + 4U * (ks / 2 / kKWords)) * kKWords + (ks / 2) % kKWords;
-    return 8U * word + 2U * (ks % 2) + b + 4U * half;
+  // K meets the query as F16 (steps of 16 dimensions) or, where its codes are integers, as INT8 (steps of 32)
+  static constexpr bool kIntegerKeys = ENC != QLLM_KV_F16;
+  static constexpr int kSteps = kIntegerKeys ? HD / 32 : HD / 16;
+  static constexpr int kPerRegister = kIntegerKeys ? 4 : 2;
+  // dimension of part `part` of fragment register b (0, 1) in step `step`, lane c.  `turn`: 2 if the words of a Q8 row
+  // begin two codes before the record does (words(), below).
+  static __device__ __forceinline__ uint32_t query_dim(int step, int b, int part, uint32_t c, uint32_t turn) {
+    if constexpr (ENC == QLLM_KV_F16) return 8U * (c + 4U * (step / 2)) + 4U * (step % 2) + 2U * b + part;
+    if constexpr (ENC == QLLM_KV_Q8) return turned(4U * (c + 4U * (2 * step + b)) + part, turn);
+    const uint32_t word = (c + 4U * (step / kKWords)) * kKWords + step % kKWords;
+    return 8U * word + 2U * part + b;
   }
   // first of the two neighbouring dimensions of output tile mt in lane r
-  static __device__ __forceinline__ uint32_t out_dim(int mt, uint32_t r) {
+  static __device__ __forceinline__ uint32_t out_dim(int mt, uint32_t r, uint32_t turn) {
     if constexpr (ENC == QLLM_KV_F16) return 8U * (r + 8U * (mt / 4)) + 2U * (mt % 4);
-    if constexpr (ENC == QLLM_KV_Q8) return 2U * (r + 8U * mt);
+    if constexpr (ENC == QLLM_KV_Q8) return turned(4U * (r + 8U * (mt / 2)) + 2U * (mt % 2), turn);
     const uint32_t word = (r + 8U * (mt / 4 / kVWords)) * kVWords + (mt / 4) % kVWords;
     return 8U * word + 2U * (mt % 4);
   }
+  static __device__ __forceinline__ uint32_t turned(uint32_t d, uint32_t turn) { return d < turn ? d + HD - turn : d - turn; }
 };
 
 // Where the keys of a 16-key block lie.
@@ -226,14 +256,16 @@ struct Cursor {
 template <typename T, int ENC, int HD>
 struct Traits {
   static constexpr bool kPrecise = sizeof(T) == 4;
-  static constexpr int kTerms = kPrecise ? 2 : 1;
-  static constexpr int kSteps = HD / 16;
+  // fragments of the query per step: F16 terms, or INT8 digits of a 21-bit integer
+  static constexpr int kTerms = Layout<ENC, HD>::kIntegerKeys ? 3 : kPrecise ? 2 : 1;
+  static constexpr int kSteps = Layout<ENC, HD>::kSteps;
   static constexpr bool kQueryInRegisters = HD <= 128;
   static constexpr int kBlocksPerSm = HD == 64 ? 4 : HD == 128 ? 3 : 2;
   // the queries of one kv head: rows 16 bytes apart from a multiple of 128 (free of bank conflicts), then fragments in their place
   static constexpr int kQueryPitch = HD * static_cast<int>(sizeof(T)) + 16;
-  static constexpr size_t kQueryBytes = static_cast<size_t>(kHeads) * kQueryPitch;
-  static_assert(kQueryBytes >= static_cast<size_t>(kSteps) * 32 * kTerms * sizeof(uint2), "fragments fit");
+  static constexpr size_t kRowsBytes = static_cast<size_t>(kHeads) * kQueryPitch;
+  static constexpr size_t kFragmentBytes = kQueryInRegisters ? 0 : static_cast<size_t>(kSteps) * 32 * kTerms * sizeof(uint2);
+  static constexpr size_t kQueryBytes = kRowsBytes > kFragmentBytes ? kRowsBytes : kFragmentBytes;
   static constexpr int kRow = HD + 4;  // floats of one head in the merge area
   static constexpr size_t kMergeBytes = (kWarps * kHeads * kRow + 2 * kWarps * kHeads) * sizeof(float);
   static constexpr size_t kRingBytes = Layout<ENC, HD>::kStaged ? static_cast<size_t>(kWarps) * Layout<ENC, HD>::kStages * Layout<ENC, HD>::kStage : 0;
@@ -311,6 +343,11 @@ __device__ __forceinline__ void weight_fragments(const float (&p)[4], uint32_t (
 __device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from, bool there) {
   const uint32_t bytes = there ? 16U : 0U;  // 0: the 16 bytes become zero and nothing is read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+template <int kOffset>
+__device__ __forceinline__ void copy16_if(bool wanted, uint32_t to, const uint8_t* from) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0+%3], [%1], 16;\n\t}" ::"r"(to), "l"(from),
+               "r"(static_cast<uint32_t>(wanted)), "n"(kOffset) : "memory");
 }
 
 __device__ __forceinline__ Block take_block(const Block& mine, int lane) {
@@ -409,29 +446,38 @@ struct Warp {
       if (b.count) load_words<1>(&scales, scales_of(b) + to_values + 4U * r);
     }
   }
+  // The three digits' products (each exact) as one FP32 score.
+  static __device__ __forceinline__ void join_digits(const int (&d)[3][4], float (&s)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      s[i] = fmaf(static_cast<float>(d[2][i]), 16384.0F, fmaf(static_cast<float>(d[1][i]), 128.0F, static_cast<float>(d[0][i])));
+  }
   template <int kQ>
   __device__ __forceinline__ void score(const uint2 (&q)[kQ], const uint32_t (&k)[L::kRegs], float (&s)[4]) const {
-    s[0] = s[1] = s[2] = s[3] = 0.0F;
+    if constexpr (ENC == QLLM_KV_F16) {
+      s[0] = s[1] = s[2] = s[3] = 0.0F;
 #pragma unroll
-    for (int w = 0; w < X::kSteps / 2; ++w) {
-      uint32_t lo[4], hi[4];
-      if constexpr (ENC == QLLM_KV_F16) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          lo[i] = k[4 * w + i];
-          hi[i] = k[HD / 8 + 4 * w + i];
-        }
-      } else {
-        nibbles_to_half(k[w], lo);
-        nibbles_to_half(k[HD / 32 + w], hi);
-      }
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int step = 0; step < X::kSteps; ++step) {
+        const int i = 2 * step;  // words 4 w, 4 w + 1 and 4 w + 2, 4 w + 3 of a chunk
 #pragma unroll
         for (int term = 0; term < X::kTerms; ++term) {
-          const uint2 f = query(q, 2 * w + half, term);
-          mma16816(s, lo[2 * half], hi[2 * half], lo[2 * half + 1], hi[2 * half + 1], f.x, f.y);
+          const uint2 f = query(q, step, term);
+          mma16816(s, k[i], k[HD / 8 + i], k[i + 1], k[HD / 8 + i + 1], f.x, f.y);
         }
+      }
+    } else {
+      // the even and the odd nibbles of a word as bytes, sixteen times their value
+      int d[3][4] = {};
+#pragma unroll
+      for (int step = 0; step < X::kSteps; ++step) {
+        const uint32_t k0 = k[step], k1 = k[HD / 32 + step];
+#pragma unroll
+        for (int digit = 0; digit < 3; ++digit) {
+          const uint2 f = query(q, step, digit);
+          mma16832(d[digit], (k0 << 4U) & 0xF0F0F0F0U, (k1 << 4U) & 0xF0F0F0F0U, k0 & 0xF0F0F0F0U, k1 & 0xF0F0F0F0U, f.x, f.y);
+        }
+      }
+      join_digits(d, s);
     }
   }
   __device__ __forceinline__ void add_values(const uint32_t (&v)[L::kRegs], const float (&p)[4]) {
@@ -472,32 +518,61 @@ struct Warp {
   // ---- through shared memory (Q8): rows of windows, key 2r in row r, key 2r + 1 in row r + 8
   // The windows of the keys one after the other over the lanes: 144 bytes in a row of one key (four lanes to a key and
   // eight keys at a time need fewer instructions, but fetch a sector twice more often: 152 us against 144 us).
-  __device__ __forceinline__ void stage(const Block& b, uint32_t to) {
-    constexpr int kCopies = (16 * L::kWindows + 31) / 32;  // of a lane, for K and for V
-    const uint8_t* base = b.keys ? b.keys : reinterpret_cast<const uint8_t*>(a.cache.page_tables);
-    const uint32_t step = b.keys ? stride : 0U, to_v = b.keys ? to_values : 0U;
+  static constexpr int kCopies = L::kStaged ? (16 * L::kWindows + 31) / 32 : 1;  // of a lane, for K and for V
+  uint32_t key_at[kCopies];    // bytes from a block's first record to that of the lane's i-th window
+  uint32_t row_at[kCopies];    // where the window goes in a stage
+  uint32_t window_at[kCopies]; // 16 * window
+  uint32_t key_shift[2], value_shift[4];  // of keys 2r, 2r + 1 and 4c .. 4c + 3: bytes from the block's first record, mod 16
+  uint32_t turn_keys, turn_values;        // byte selectors that put the tail in the place of a turned row's first two bytes
+  __device__ __forceinline__ void layout_staged() {
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
       const uint32_t index = lane + 32U * i, key = index / L::kWindows, window = index % L::kWindows;
-      if (index >= 16U * L::kWindows) break;
-      const bool there = key < b.count;  // else zeros, and the address only has to be one that exists
+      key_at[i] = key * stride;
+      row_at[i] = (key / 2U + 8U * (key & 1U)) * L::kPitch + 16U * window;
+      window_at[i] = 16U * window;
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < 2U; ++k) key_shift[k] = (2U * r + k) * stride & 15U;
+#pragma unroll
+    for (uint32_t k = 0; k < 4U; ++k) value_shift[k] = (4U * c + k) * stride & 15U;
+  }
+  __device__ __forceinline__ void stage(const Block& b, uint32_t to) {
+    if (b.count == 16U) {
+      const uintptr_t base = reinterpret_cast<uintptr_t>(b.keys) & ~static_cast<uintptr_t>(15U);
+      const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(b.keys)) & 15U;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(base) + (((shift + key_at[i]) & ~15U) + window_at[i]);
+        const bool wanted = i + 1 < kCopies || 16 * L::kWindows % 32 == 0 || lane < 16U * L::kWindows % 32U;
+        copy16_if<0>(wanted, to + row_at[i], from);
+        copy16_if<16 * L::kPitch>(wanted, to + row_at[i], from + to_values);  // V begins on 16 bytes
+      }
+      return;
+    }
+    // keys that do not count become zeros, and their address only has to be one that exists
+    const uint8_t* base = b.keys ? b.keys : reinterpret_cast<const uint8_t*>(a.cache.page_tables);
+    const uint32_t step = b.keys ? stride : 0U, to_v = b.keys ? to_values : 0U;
+    for (uint32_t index = lane; index < 16U * L::kWindows; index += 32U) {
+      const uint32_t key = index / L::kWindows, window = index % L::kWindows;
       const uint8_t* from =
           reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(base + key * step) & ~static_cast<uintptr_t>(15U)) + 16U * window;
       const uint32_t row = to + (key / 2U + 8U * (key & 1U)) * L::kPitch + 16U * window;
-      copy16(row, from, there);
-      copy16(row + 16U * L::kPitch, from + to_v, there);  // V begins on 16 bytes
+      copy16(row, from, key < b.count);
+      copy16(row + 16U * L::kPitch, from + to_v, key < b.count);
     }
   }
-  // where a record begins in its row (K and V alike; pages and layers begin on 16 bytes)
-  __device__ __forceinline__ uint32_t shift_of(const Block& b, uint32_t key) const {
-    return (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(b.keys)) + key * stride) & 15U;
+  // What is left to know of a staged block: keys that count, and where its first record begins in its row.
+  static __device__ __forceinline__ uint32_t staged_as(const Block& b) {
+    return b.count << 4U | (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(b.keys)) & 15U);
   }
 
   // The warp's part of tokens [first, last) of the sequence: every `phases`-th block of 16 from `phase` on.  begin() starts
   // the first loads, which need no query; tokens() does the rest.
   struct Start {
     uint32_t k[L::kStaged ? 1 : kN][L::kRegs], v[L::kStaged ? 1 : kN][L::kRegs], kscale[L::kStaged ? 1 : kN], vscale[L::kStaged ? 1 : kN];
-    Block now[L::kStaged ? L::kStages : kN];
+    Block now[L::kStaged ? 1 : kN];
+    uint32_t staged[L::kStages - 1];  // of the tiles on their way
     Block ahead;
     uint32_t tiles;
   };
@@ -518,9 +593,10 @@ struct Warp {
     } else {
 #pragma unroll
       for (int i = 0; i < L::kStages - 1; ++i) {
-        x.now[i] = block_at(at, last);
+        const Block b = block_at(at, last);
         at.advance(a.cache);
-        if (static_cast<uint32_t>(i) < x.tiles) stage(x.now[i], ring + i * L::kStage);
+        x.staged[i] = staged_as(b);
+        if (static_cast<uint32_t>(i) < x.tiles) stage(b, ring + i * L::kStage);
         asm volatile("cp.async.commit_group;" ::: "memory");
       }
     }
@@ -529,7 +605,7 @@ struct Warp {
   }
   template <int kQ>
   __device__ __forceinline__ void tokens(Start& x, Cursor& at, const uint2 (&q)[kQ], uint32_t first, uint32_t last, uint32_t phase, uint32_t phases,
-                                         float* scores, size_t capacity, uint32_t heads_here, uint8_t* ring) {
+                                         float* scores, size_t capacity, uint32_t heads_here, uint32_t ring) {
     if constexpr (!L::kStaged) {
       for (uint32_t tile = 0; tile < x.tiles; ++tile) {
         float s[kN][4], vs[kN][2];
@@ -538,11 +614,24 @@ struct Warp {
         for (int b = 0; b < kN; ++b) {
           score(q, x.k[b], s[b]);
           count[b] = x.now[b].count;
-          const float2 ks = ENC == QLLM_KV_Q4H ? unpack_half(x.kscale[b]) : make_float2(1.0F, 1.0F);
+          if constexpr (ENC == QLLM_KV_Q4H) {
+            const float2 ks = unpack_half(x.kscale[b]);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            s[b][h] = 2U * r < count[b] ? s[b][h] * (ks.x * scale[h]) : -INFINITY;
-            s[b][2 + h] = 2U * r + 1U < count[b] ? s[b][2 + h] * (ks.y * scale[h]) : -INFINITY;
+            for (int h = 0; h < 2; ++h) {
+              s[b][h] *= ks.x * scale[h];
+              s[b][2 + h] *= ks.y * scale[h];
+            }
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              s[b][h] *= scale[h];
+              s[b][2 + h] *= scale[h];
+            }
+          }
+          if (count[b] < 16U) {
+#pragma unroll
+            for (uint32_t k = 0; k < 2U; ++k)
+              if (2U * r + k >= count[b]) s[b][2 * k] = s[b][2 * k + 1] = -INFINITY;
           }
           if (scores) put_scores(scores, capacity, heads_here, first + 16U * (phase + phases * (tile * kN + b)), last, s[b]);
         }
@@ -557,8 +646,12 @@ struct Warp {
 #pragma unroll
         for (int b = 0; b < kN; ++b) {
           const float2 f = ENC == QLLM_KV_Q4H ? unpack_half(x.vscale[b]) : make_float2(1.0F, 1.0F);
-          vs[b][0] = 2U * r < count[b] ? f.x : 0.0F;
-          vs[b][1] = 2U * r + 1U < count[b] ? f.y : 0.0F;
+          vs[b][0] = f.x;
+          vs[b][1] = f.y;
+          if (count[b] < 16U) {
+            if (2U * r >= count[b]) vs[b][0] = 0.0F;
+            if (2U * r + 1U >= count[b]) vs[b][1] = 0.0F;
+          }
         }
         softmax_tile<HD, kN, ENC != QLLM_KV_F16>(run, s, vs);
 #pragma unroll
@@ -570,88 +663,133 @@ struct Warp {
           at.advance(a.cache);
         }
       }
+    } else if (a.cache.kv_heads & 1U) {
+      staged_tokens<true>(x, at, q, first, last, phase, phases, scores, capacity, heads_here, ring);
     } else {
-      const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-      for (uint32_t tile0 = 0; tile0 < x.tiles; tile0 += L::kStages) {
-#pragma unroll
-        for (int i = 0; i < L::kStages; ++i) {
-          const uint32_t tile = tile0 + i;
-          if (tile >= x.tiles) break;
-          asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
-          __syncwarp();
-          staged_block(q, x.now[i], ring + i * L::kStage, first + 16U * (phase + phases * tile), last, scores, capacity, heads_here);
-          __syncwarp();
-          constexpr int kBehind = L::kStages - 1;
-          x.now[(i + kBehind) % L::kStages] = x.ahead;
-          if (tile + kBehind < x.tiles) stage(x.ahead, base + (i + kBehind) % L::kStages * L::kStage);
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          x.ahead = block_at(at, last);
-          at.advance(a.cache);
-        }
-      }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      staged_tokens<false>(x, at, q, first, last, phase, phases, scores, capacity, heads_here, ring);
     }
   }
-  __device__ __forceinline__ void put_scores(float* scores, size_t capacity, uint32_t heads_here, uint64_t token, uint32_t last,
+  template <bool kAlternate, int kQ>
+  __device__ __forceinline__ void staged_tokens(Start& x, Cursor& at, const uint2 (&q)[kQ], uint32_t first, uint32_t last, uint32_t phase,
+                                                uint32_t phases, float* scores, size_t capacity, uint32_t heads_here, uint32_t ring) {
+    // not unrolled over the stages: the loop is some 450 instructions, and three copies of it waited for instructions
+    uint32_t here = ring, there = ring + (L::kStages - 1) * L::kStage;  // of this tile, and of the one staged next
+#pragma unroll 1
+    for (uint32_t tile = 0; tile < x.tiles; ++tile) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
+      __syncwarp();  // everybody's copies have arrived, and the tile before has been read
+      const uint32_t staged = x.staged[0];
+#pragma unroll
+      for (int i = 0; i + 2 < L::kStages; ++i) x.staged[i] = x.staged[i + 1];
+      x.staged[L::kStages - 2] = staged_as(x.ahead);
+      if (tile + L::kStages - 1U < x.tiles) stage(x.ahead, there);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      x.ahead = block_at(at, last);
+      at.advance(a.cache);
+      staged_block<kAlternate>(q, staged, here, first + 16U * (phase + phases * tile), last, scores, capacity, heads_here);
+      there = here;
+      here = here + L::kStage == ring + L::kStages * L::kStage ? ring : here + L::kStage;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
+  // `token`: of the block's first key; the scores of keys that lie on no page are -inf and belong there too
+  __device__ __forceinline__ void put_scores(float* scores, size_t capacity, uint32_t heads_here, uint32_t token, uint32_t last,
                                              const float (&s)[4]) const {
+    float* to = scores + 2U * c * capacity + token + 2U * r;
+    if (token + 16U <= last) {  // rows of scores hold a multiple of 16, blocks begin at one
+      if (2U * c < heads_here) *reinterpret_cast<float2*>(to) = make_float2(s[0], s[2]);
+      if (2U * c + 1U < heads_here) *reinterpret_cast<float2*>(to + capacity) = make_float2(s[1], s[3]);
+      return;
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (2U * c + h >= heads_here) continue;
-      float* to = scores + (2U * c + h) * capacity + token + 2U * r;
-      if (token + 2U * r < last) to[0] = s[h];
-      if (token + 2U * r + 1U < last) to[1] = s[2 + h];
+      if (token + 2U * r < last) to[h * capacity] = s[h];
+      if (token + 2U * r + 1U < last) to[h * capacity + 1U] = s[2 + h];
     }
   }
-  template <int kQ>
-  __device__ __forceinline__ void staged_block(const uint2 (&q)[kQ], const Block& b, const uint8_t* at, uint32_t token, uint32_t last,
+  // The codes of a staged record in words, word x + kLanes * i for lane x of the kLanes that share the row.  A record begins on
+  // a 2-byte boundary, and the words are those of memory: where the first holds the two bytes before the record, the one
+  // behind the last full word (`tail`) has the last two codes.  Those take the place of the first two bytes (`selector`): the
+  // lane then holds the dimensions turned round by two, the same for every key of a head when kv_heads is even.  When it is
+  // odd, records begin one way and the other in turn, and the words of the odd ones are put together anew (`realign`).
+  template <int kLanes, bool kAlternate, int kN2>
+  __device__ __forceinline__ void words(uint32_t record, uint32_t x, bool realign, uint32_t selector, uint32_t (&w)[kN2], uint32_t& tail) const {
+    constexpr int kApart = kLanes == 4 ? 1 : 4;  // lanes from x to x + 1
+    const uint32_t from = record & ~3U;
+    shared_words<4 * kLanes>(from + 4U * x, w);
+    tail = shared_word<HD>(from);
+    if constexpr (kAlternate) {
+      if (!realign) return;
+#pragma unroll
+      for (int i = 0; i < kN2; ++i) {
+        const uint32_t beside = __shfl_sync(0xffffffffU, w[i], lane + kApart);
+        const uint32_t around = i + 1 < kN2 ? __shfl_sync(0xffffffffU, w[(i + 1) % kN2], lane - kApart * (kLanes - 1)) : tail;
+        w[i] = __funnelshift_r(w[i], x + 1U < kLanes ? beside : around, 16U);
+      }
+    } else {
+      w[0] = __byte_perm(w[0], tail, selector);
+    }
+  }
+  template <bool kAlternate, int kQ>
+  __device__ __forceinline__ void staged_block(const uint2 (&q)[kQ], uint32_t staged, uint32_t at, uint32_t token, uint32_t last,
                                                float* scores, size_t capacity, uint32_t heads_here) {
-    float s[1][4] = {{0.0F, 0.0F, 0.0F, 0.0F}}, vs[1][2], ks[2];
-    const uint8_t* rows[2];
+    const uint32_t count = staged >> 4U, shift = staged & 15U;
+    float s[1][4], vs[1][2], ks[2];
+    uint32_t w[2][HD / 16];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      rows[k] = at + (r + 8U * k) * L::kPitch + shift_of(b, 2U * r + k);
-      ks[k] = __half2float(*reinterpret_cast<const __half*>(rows[k] + HD));
-      const uint8_t* value = at + (16U + r + 8U * k) * L::kPitch + shift_of(b, 2U * r + k);
-      vs[0][k] = 2U * r + k < b.count ? __half2float(*reinterpret_cast<const __half*>(value + HD)) : 0.0F;
+      const uint32_t row = at + (r + 8U * k) * L::kPitch + ((shift + key_shift[k]) & 15U);
+      const bool odd = (kv_head + (kAlternate ? k : 0)) & 1U;
+      uint32_t tail;
+      words<4, kAlternate>(row, c, odd, turn_keys, w[k], tail);
+      ks[k] = __half2float(__ushort_as_half(static_cast<unsigned short>(odd ? tail >> 16U : tail)));
+      vs[0][k] = shared_half<16 * L::kPitch + HD>(row);
     }
+    {
+      int d[3][4] = {};
 #pragma unroll
-    for (int step = 0; step < X::kSteps; ++step) {
-      uint32_t x[2][2];
+      for (int step = 0; step < X::kSteps; ++step)
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t pair = *reinterpret_cast<const uint16_t*>(rows[k] + 2U * (c + 4U * (2 * step + half)));
-          x[k][half] = bytes_to_half(__byte_perm(pair, 0U, 0x4140));
+        for (int digit = 0; digit < 3; ++digit) {
+          const uint2 f = query(q, step, digit);
+          mma16832(d[digit], w[0][2 * step], w[1][2 * step], w[0][2 * step + 1], w[1][2 * step + 1], f.x, f.y);
         }
-#pragma unroll
-      for (int term = 0; term < X::kTerms; ++term) {
-        const uint2 f = query(q, step, term);
-        mma16816(s[0], x[0][0], x[1][0], x[0][1], x[1][1], f.x, f.y);
-      }
+      join_digits(d, s[0]);
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) s[0][2 * k + h] = 2U * r + k < b.count ? s[0][2 * k + h] * (ks[k] * scale[h]) : -INFINITY;
+      for (int h = 0; h < 2; ++h) s[0][2 * k + h] *= ks[k] * scale[h];
+    if (count < 16U) {
+#pragma unroll
+      for (uint32_t k = 0; k < 2U; ++k)
+        if (2U * r + k >= count) {
+          s[0][2 * k] = s[0][2 * k + 1] = -INFINITY;
+          vs[0][k] = 0.0F;
+        }
+    }
     if (scores) put_scores(scores, capacity, heads_here, token, last, s[0]);
     softmax_tile<HD, 1, true>(run, s, vs);
     uint32_t hi[2], lo[2] = {0U, 0U};
     weight_fragments<X::kPrecise>(s[0], hi, lo);
-    const uint8_t* v[4];
+    uint32_t v[4][HD / 32];
 #pragma unroll
-    for (uint32_t k = 0; k < 4U; ++k)
-      v[k] = at + (16U + 2U * c + k / 2U + 8U * (k & 1U)) * L::kPitch + shift_of(b, 4U * c + k) + 2U * r;
-#pragma unroll
-    for (int mt = 0; mt < HD / 16; ++mt) {
-      uint32_t x[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint16_t*>(v[k] + 16 * mt);
-      const uint32_t even = __byte_perm(x[0], x[2], 0x5410), odd = __byte_perm(x[1], x[3], 0x5410);
-      const uint32_t a0 = bytes_to_half(even), a1 = bytes_to_half(even >> 8U), a2 = bytes_to_half(odd), a3 = bytes_to_half(odd >> 8U);
-      mma16816(run.out[mt], a0, a1, a2, a3, hi[0], hi[1]);
-      if constexpr (X::kPrecise) mma16816(run.out[mt], a0, a1, a2, a3, lo[0], lo[1]);
+    for (uint32_t k = 0; k < 4U; ++k) {
+      uint32_t tail;
+      words<8, kAlternate>(at + (16U + 2U * c + k / 2U + 8U * (k & 1U)) * L::kPitch + ((shift + value_shift[k]) & 15U), r,
+                           (kv_head + (kAlternate ? k : 0U)) & 1U, turn_values, v[k], tail);
     }
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t selector = half ? 0x7632U : 0x5410U;
+        const uint32_t even = __byte_perm(v[0][j], v[2][j], selector), odd = __byte_perm(v[1][j], v[3][j], selector);
+        const uint32_t a0 = bytes_to_half(even), a1 = bytes_to_half(even >> 8U), a2 = bytes_to_half(odd), a3 = bytes_to_half(odd >> 8U);
+        mma16816(run.out[2 * j + half], a0, a1, a2, a3, hi[0], hi[1]);
+        if constexpr (X::kPrecise) mma16816(run.out[2 * j + half], a0, a1, a2, a3, lo[0], lo[1]);
+      }
   }
 };
 
@@ -713,10 +851,11 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
 
   using W = Warp<T, ENC, HD>;
   W w{a};
-  w.layout();
   w.lane = lane;
   w.r = lane >> 2U;
   w.c = lane & 3U;
+  w.layout();
+  if constexpr (L::kStaged) w.layout_staged();
   const uint32_t in_set = warp % plan.heads, phase = warp / plan.heads, phases = kWarps / plan.heads;
   uint2* fragments = reinterpret_cast<uint2*>(shared + in_set * X::kQueryBytes);
   uint8_t* area = shared + X::kQueryBytes * plan.heads;
@@ -748,13 +887,15 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
 
     w.sequence = s;
     w.kv_head = kv_head;
-    uint8_t* ring = area + warp * (L::kStages * L::kStage);
-    const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(area)) + warp * (L::kStages * L::kStage);
+    const uint32_t turn = ENC == QLLM_KV_Q8 && !(a.cache.kv_heads & 1U) ? 2U * (kv_head & 1U) : 0U;  // see words()
+    w.turn_keys = turn && w.c == 0U ? 0x3254U : 0x3210U;
+    w.turn_values = turn && w.r == 0U ? 0x3254U : 0x3210U;
     Cursor at(a.cache, first + 16U * (phase + phases * (L::kStaged ? 0U : lane % W::kN)), 16U * phases * W::kN);
     typename W::Start x;
     __syncthreads();  // the merge area and the queries of the item before have been read
     // the first keys are on their way while the query is made ready (where it leaves room in the registers)
-    if constexpr (X::kQueryInRegisters) w.begin(x, at, first, last, phase, phases, ring_at);
+    if constexpr (X::kQueryInRegisters) w.begin(x, at, first, last, phase, phases, ring);
 
     // ---- the query heads as fragments, scaled to [2^8, 2^9)
     constexpr uint32_t kChunks = kHeads * HD * sizeof(T) / 16U, kRowChunks = HD * sizeof(T) / 16U;
@@ -767,21 +908,30 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
     }
     __syncthreads();
     const T* row = reinterpret_cast<const T*>(shared + in_set * X::kQueryBytes + w.r * X::kQueryPitch);
-    float value[X::kSteps][2][2];
+    constexpr int kPer = L::kPerRegister;
+    float value[X::kSteps][2][kPer];
     float top = 0.0F;
+    bool wrong = false;  // a NaN, or (INT8) an infinity
 #pragma unroll
     for (int step = 0; step < X::kSteps; ++step)
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          value[step][b][half] = row_value(row[L::query_dim(step, b, half, w.c)]);
-          top = fmaxf(top, fabsf(value[step][b][half]));
+        for (int part = 0; part < kPer; ++part) {
+          const float x0 = row_value(row[L::query_dim(step, b, part, w.c, turn)]);
+          value[step][b][part] = x0;
+          wrong = wrong || !(fabsf(x0) < INFINITY);
+          top = fmaxf(top, fabsf(x0));
         }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 2));
-    const int up = top > 0.0F && top < INFINITY ? 8 - ilogbf(top) : 0;
-    const float unit = ldexpf(a.scale * kLog2e, -up);  // of head r
+    // F16: to [2^8, 2^9); INT8 digits: to [2^19, 2^20)
+    const int up = top > 0.0F && top < INFINITY ? (L::kIntegerKeys ? 19 : 8) - ilogbf(top) : 0;
+    float unit = ldexpf(a.scale * kLog2e, -up - (ENC == QLLM_KV_Q4H ? 4 : 0));  // of head r; Q4H codes come times sixteen
+    if constexpr (L::kIntegerKeys) {
+      const uint32_t lanes = __ballot_sync(0xffffffffU, wrong);
+      if (lanes >> (4U * w.r) & 15U) unit = NAN;  // integers would lose it
+    }
     w.scale[0] = __shfl_sync(0xffffffffU, unit, 8U * w.c);
     w.scale[1] = __shfl_sync(0xffffffffU, unit, 8U * w.c + 4U);
     // two factors: one may not be a float by itself
@@ -790,25 +940,35 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
     if constexpr (!X::kQueryInRegisters) __syncthreads();  // the fragments take the queries' place
 #pragma unroll
     for (int step = 0; step < X::kSteps; ++step) {
-      uint32_t hi[2], lo[2];
+      uint32_t term[3][2] = {};
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const float x0 = value[step][b][0] * up0 * up1, x1 = value[step][b][1] * up0 * up1;
-        hi[b] = pack_half(x0, x1);
-        const float2 f = unpack_half(hi[b]);
-        lo[b] = pack_half(x0 - f.x, x1 - f.y);
+        if constexpr (L::kIntegerKeys) {
+#pragma unroll
+          for (int part = 0; part < kPer; ++part) {
+            // three balanced digits of base 128
+            const int n = __float2int_rn(value[step][b][part] * up0 * up1);
+            const int d0 = ((n + 64) & 127) - 64, n1 = (n - d0) >> 7, d1 = ((n1 + 64) & 127) - 64, d2 = (n1 - d1) >> 7;
+            term[0][b] |= (static_cast<uint32_t>(d0) & 255U) << (8 * part);
+            term[1][b] |= (static_cast<uint32_t>(d1) & 255U) << (8 * part);
+            term[2][b] |= (static_cast<uint32_t>(d2) & 255U) << (8 * part);
+          }
+        } else {
+          const float x0 = value[step][b][0] * up0 * up1, x1 = value[step][b][1] * up0 * up1;
+          term[0][b] = pack_half(x0, x1);
+          const float2 f = unpack_half(term[0][b]);
+          term[1][b] = pack_half(x0 - f.x, x1 - f.y);
+        }
       }
-      if constexpr (X::kQueryInRegisters) {
-        q[step * X::kTerms] = make_uint2(hi[0], hi[1]);
-        if constexpr (X::kPrecise) q[step * X::kTerms + 1] = make_uint2(lo[0], lo[1]);
-      } else if (phase == 0U) {
-        fragments[step * X::kTerms * 32 + lane] = make_uint2(hi[0], hi[1]);
-        if constexpr (X::kPrecise) fragments[(step * X::kTerms + 1) * 32 + lane] = make_uint2(lo[0], lo[1]);
+#pragma unroll
+      for (int i = 0; i < X::kTerms; ++i) {
+        if constexpr (X::kQueryInRegisters) q[step * X::kTerms + i] = make_uint2(term[i][0], term[i][1]);
+        else if (phase == 0U) fragments[(step * X::kTerms + i) * 32 + lane] = make_uint2(term[i][0], term[i][1]);
       }
     }
     if constexpr (!X::kQueryInRegisters) {
       __syncthreads();
-      w.begin(x, at, first, last, phase, phases, ring_at);
+      w.begin(x, at, first, last, phase, phases, ring);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -835,7 +995,7 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
       }
 #pragma unroll
       for (int mt = 0; mt < HD / 16; ++mt)
-        *reinterpret_cast<float2*>(merge_out + row * X::kRow + L::out_dim(mt, w.r)) = make_float2(w.run.out[mt][h], w.run.out[mt][2 + h]);
+        *reinterpret_cast<float2*>(merge_out + row * X::kRow + L::out_dim(mt, w.r, turn)) = make_float2(w.run.out[mt][h], w.run.out[mt][2 + h]);
     }
     __syncthreads();
     const bool begins = from == 0U, whole = begins && last == length;
@@ -845,32 +1005,33 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
           make_uint2(blockIdx.x, static_cast<uint32_t>(((last_unit + 1ULL) * blocks - 1ULL) / total));
     }
     float* place = plan.partials + (static_cast<size_t>(blockIdx.x) * 2U + (begins ? 1U : 0U)) * plan.place;
-    for (uint32_t e = threadIdx.x; e < plan.heads * heads_here * HD; e += kThreads) {
-      const uint32_t d = e % HD, g = e / HD % heads_here, h = e / HD / heads_here;
-      float top = -INFINITY;
-      for (uint32_t p = 0; p < phases; ++p) top = fmaxf(top, merge_max[(p * plan.heads + h) * kHeads + g]);
-      float sum = 0.0F, out = 0.0F;
-      if (top != -INFINITY)
+    for (uint32_t h = 0; h < plan.heads; ++h)
+      for (uint32_t e = threadIdx.x; e < heads_here * HD; e += kThreads) {
+        const uint32_t d = e % HD, g = e / HD;
+        float top = -INFINITY;
+        for (uint32_t p = 0; p < phases; ++p) top = fmaxf(top, merge_max[(p * plan.heads + h) * kHeads + g]);
+        const float reference = top == -INFINITY ? 0.0F : top;
+        float sum = 0.0F, out = 0.0F;
         for (uint32_t p = 0; p < phases; ++p) {
           const uint32_t row = (p * plan.heads + h) * kHeads + g;
-          const float f = exp2_fast(merge_max[row] - top);
-          sum = fmaf(merge_sum[row], f, sum);
+          const float f = exp2_fast(merge_max[row] - reference);
+          sum = fmaf(merge_sum[row], f, sum);  // 0 where no key counts, NaN where a score was NaN
           out = fmaf(merge_out[row * X::kRow + d], f, out);
         }
-      const uint32_t head = (set * plan.heads + h) * plan.group + tile * kHeads + g;
-      if (whole) {
-        put_row(static_cast<T*>(a.out) + static_cast<size_t>(s) * a.out_stride + static_cast<size_t>(head) * HD + d,
-                top == -INFINITY ? 0.0F : out / sum);
-        if (plan.lse && d == 0U) plan.lse[static_cast<size_t>(s) * a.q_heads + head] = top == -INFINITY ? 0.0F : top + log2f(sum);
-      } else {
-        const uint32_t row = h * kHeads + g;
-        place[2U * plan.rows + row * HD + d] = out;
-        if (d == 0U) {
-          place[row] = top;
-          place[plan.rows + row] = sum;
+        const uint32_t head = (set * plan.heads + h) * plan.group + tile * kHeads + g;
+        if (whole) {
+          put_row(static_cast<T*>(a.out) + static_cast<size_t>(s) * a.out_stride + static_cast<size_t>(head) * HD + d,
+                  sum == 0.0F ? 0.0F : out / sum);
+          if (plan.lse && d == 0U) plan.lse[static_cast<size_t>(s) * a.q_heads + head] = sum == 0.0F ? 0.0F : reference + log2f(sum);
+        } else {
+          const uint32_t row = h * kHeads + g;
+          place[2U * plan.rows + row * HD + d] = out;
+          if (d == 0U) {
+            place[row] = top;
+            place[plan.rows + row] = sum;
+          }
         }
       }
-    }
     u += take;
   }
 }
@@ -944,10 +1105,10 @@ __device__ __forceinline__ void join_head(const DecodeAttentionArgs& a, const Pl
       float total = 0.0F;
 #pragma unroll
       for (uint32_t w = 0; w < kWays; ++w) total += reinterpret_cast<const float*>(part[w])[d];
-      put_row(out + d, top == -INFINITY ? 0.0F : total / sum);
+      put_row(out + d, sum == 0.0F ? 0.0F : total / sum);
     }
   } else {
-    const float scale = top == -INFINITY ? 0.0F : 1.0F / sum;
+    const float scale = sum == 0.0F ? 0.0F : 1.0F / sum;
 #pragma unroll
     for (uint32_t v = 0; v < kVectors; ++v) {
       if (lane + 32U * v >= HD / 4) continue;
@@ -979,12 +1140,12 @@ __device__ __forceinline__ void add_weights(const DecodeAttentionArgs& a, const 
       } else {
         const uint32_t place_row = (h % plan.heads) * kHeads + g;
         const float top = top_of(plan, span, place_row, lane);
+        const float reference = top == -INFINITY ? 0.0F : top;
         float total = 0.0F;
-        if (top != -INFINITY)
-          for (uint32_t i = lane; i < span.y - span.x + 1U; i += 32U)
-            total += place_of(plan, span, i)[plan.rows + place_row] * exp2_fast(place_of(plan, span, i)[place_row] - top);
+        for (uint32_t i = lane; i < span.y - span.x + 1U; i += 32U)
+          total += place_of(plan, span, i)[plan.rows + place_row] * exp2_fast(place_of(plan, span, i)[place_row] - reference);
         total = warp_sum(total);
-        value = top == -INFINITY ? 0.0F : top + log2f(total);
+        value = total == 0.0F ? 0.0F : reference + log2f(total);
       }
       if (lane == 0U) lse[g] = value;
     }

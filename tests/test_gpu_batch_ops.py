@@ -208,7 +208,8 @@ ATTENTION_CASES = [
     (40, 8, 128, BF16, F16, 256), (40, 8, 128, BF16, Q4H, 256), (40, 8, 128, HF16, Q8, 256), (32, 4, 128, HF16, F16, 64),
     (16, 16, 64, F32, F16, 16), (4, 2, 64, BF16, Q8, 48), (6, 1, 64, HF16, Q4H, 16), (12, 2, 256, F32, Q4H, 64),
     (12, 1, 128, BF16, F16, 48), (16, 1, 256, HF16, F16, 16), (24, 1, 192, F32, Q8, 96), (3, 1, 192, BF16, Q4H, 32), (5, 5, 256, BF16, Q8, 16),
-    (17, 1, 128, F32, F16, 256), (8, 1, 128, F32, Q4H, 16), (10, 5, 64, F32, Q8, 768), (9, 3, 192, HF16, F16, 48), (6, 6, 192, F32, Q4H, 16)]
+    (17, 1, 128, F32, F16, 256), (8, 1, 128, F32, Q4H, 16), (10, 5, 64, F32, Q8, 768), (9, 3, 192, HF16, F16, 48), (6, 6, 192, F32, Q4H, 16),
+    (8, 2, 192, F32, Q8, 16), (4, 4, 256, BF16, Q8, 48), (6, 3, 128, HF16, Q8, 32)]   # Q8 records: even and odd numbers of heads
 
 
 @pytest.mark.parametrize("q,kv,hd,dtype,enc,page", ATTENTION_CASES)
@@ -340,6 +341,35 @@ def test_attention_long(q, kv, hd, enc, n, dtype):
     check_attention(cache, query, [1, n], q, hd ** -0.5, out, None, w_out, dtype)
     # every query head's weights sum to one
     assert torch.allclose(w_out[1, :, :n].double().sum(-1), torch.full((kv,), float(q // kv), dtype=torch.float64, device="cuda"), rtol=1e-4)
+
+
+@pytest.mark.parametrize("enc", [F16, Q4H, Q8])
+@pytest.mark.parametrize("dtype", [F32, BF16, HF16])
+def test_attention_passes_nan_and_infinity_on(enc, dtype):
+    """A NaN or an infinity in a query head makes that head NaN and its kv head's weights, nothing else; one in a key's record
+    makes every head that reads it NaN.  One long sequence (joined parts) and one short one."""
+    q, kv, hd, page, lengths = 8, 2, 128, 64, [9000, 40, 40]
+    cache = PagedCache(3, 9000 // page + 1, page, enc, kv, hd, seed=6)
+    query = rand((3, q * hd), 5).to(dtype)
+    query[0, 1 * hd + 5] = float("nan")                  # head 1 of kv head 0
+    query[1, 6 * hd + 7] = float("inf")                  # head 6 of kv head 1
+    at = cache.index[2, 0]                              # sequence 2: key 13 of kv head 1
+    if enc == F16:
+        cache.pool.view(HF16).view(-1, 2, page, kv, hd)[at, 0, 13, 1, 3] = float("nan")
+    else:
+        record = 13 * kv + 1 if enc == Q8 else 1 * page + 13
+        list(cache_scales(cache))[0][1][at, record] = float("nan")
+    out = torch.zeros((3, q * hd), dtype=dtype, device="cuda")
+    w_out = torch.full((3, kv, cache.capacity), -3.0, device="cuda")
+    bc.decode_attention(cache, query, u32(lengths), q, 0.1, out, None, w_out)
+    torch.cuda.synchronize()
+    heads = out.view(3, q, hd)
+    bad = torch.zeros(3, q, dtype=torch.bool, device="cuda")
+    bad[0, 1] = bad[1, 6] = True
+    bad[2, 4:] = True
+    assert bool(heads[bad].isnan().all()) and bool(heads[~bad].isfinite().all())
+    for s, h in ((0, 0), (1, 1), (2, 1)):
+        assert bool(w_out[s, h, :lengths[s]].isnan().all()) and bool(w_out[s, 1 - h, :lengths[s]].isfinite().all())
 
 
 def test_attention_many_short_sequences():
