@@ -264,8 +264,10 @@ struct Traits {
   // the queries of one kv head: rows 16 bytes apart from a multiple of 128 (free of bank conflicts), then fragments in their place
   static constexpr int kQueryPitch = HD * static_cast<int>(sizeof(T)) + 16;
   static constexpr size_t kRowsBytes = static_cast<size_t>(kHeads) * kQueryPitch;
-  static constexpr size_t kFragmentBytes = kQueryInRegisters ? 0 : static_cast<size_t>(kSteps) * 32 * kTerms * sizeof(uint2);
-  static constexpr size_t kQueryBytes = kRowsBytes > kFragmentBytes ? kRowsBytes : kFragmentBytes;
+  // Fragments go through shared memory where four warps share them and each makes a quarter, and where they stay there.
+  static constexpr bool kSharedQuery = !Layout<ENC, HD>::kStaged;
+  static constexpr size_t kFragmentBytes = kSharedQuery || !kQueryInRegisters ? static_cast<size_t>(kSteps) * 32 * kTerms * sizeof(uint2) : 0;
+  static constexpr size_t kQueryBytes = kSharedQuery ? kRowsBytes + kFragmentBytes : kRowsBytes > kFragmentBytes ? kRowsBytes : kFragmentBytes;
   static constexpr int kRow = HD + 4;  // floats of one head in the merge area
   static constexpr size_t kMergeBytes = (kWarps * kHeads * kRow + 2 * kWarps * kHeads) * sizeof(float);
   static constexpr size_t kRingBytes = Layout<ENC, HD>::kStaged ? static_cast<size_t>(kWarps) * Layout<ENC, HD>::kStages * Layout<ENC, HD>::kStage : 0;
@@ -857,7 +859,7 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
   w.layout();
   if constexpr (L::kStaged) w.layout_staged();
   const uint32_t in_set = warp % plan.heads, phase = warp / plan.heads, phases = kWarps / plan.heads;
-  uint2* fragments = reinterpret_cast<uint2*>(shared + in_set * X::kQueryBytes);
+  uint2* fragments = reinterpret_cast<uint2*>(shared + in_set * X::kQueryBytes + (X::kSharedQuery ? X::kRowsBytes : 0));
   uint8_t* area = shared + X::kQueryBytes * plan.heads;
   float* merge_max = reinterpret_cast<float*>(area);           // [warp][head]
   float* merge_sum = merge_max + kWarps * kHeads;
@@ -909,20 +911,14 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
     __syncthreads();
     const T* row = reinterpret_cast<const T*>(shared + in_set * X::kQueryBytes + w.r * X::kQueryPitch);
     constexpr int kPer = L::kPerRegister;
-    float value[X::kSteps][2][kPer];
     float top = 0.0F;
-    bool wrong = false;  // a NaN, or (INT8) an infinity
+    bool wrong = false;  // a NaN or an infinity
 #pragma unroll
-    for (int step = 0; step < X::kSteps; ++step)
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int part = 0; part < kPer; ++part) {
-          const float x0 = row_value(row[L::query_dim(step, b, part, w.c, turn)]);
-          value[step][b][part] = x0;
-          wrong = wrong || !(fabsf(x0) < INFINITY);
-          top = fmaxf(top, fabsf(x0));
-        }
+    for (int i = 0; i < HD / 4; ++i) {  // the row's values over its four lanes
+      const float x0 = row_value(row[4 * i + w.c]);
+      wrong = wrong || !(fabsf(x0) < INFINITY);
+      top = fmaxf(top, fabsf(x0));
+    }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 2));
     // F16: to [2^8, 2^9); INT8 digits: to [2^19, 2^20)
@@ -936,40 +932,67 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
     w.scale[1] = __shfl_sync(0xffffffffU, unit, 8U * w.c + 4U);
     // two factors: one may not be a float by itself
     const float up0 = ldexpf(1.0F, up / 2), up1 = ldexpf(1.0F, up - up / 2);
-    uint2 q[X::kQueryInRegisters ? X::kSteps * X::kTerms : 1];
-    if constexpr (!X::kQueryInRegisters) __syncthreads();  // the fragments take the queries' place
-#pragma unroll
-    for (int step = 0; step < X::kSteps; ++step) {
+    const auto make_terms = [&](int step, uint2 (&made)[3]) {
       uint32_t term[3][2] = {};
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
+        float x[kPer];
+#pragma unroll
+        for (int part = 0; part < kPer; ++part) x[part] = row_value(row[L::query_dim(step, b, part, w.c, turn)]) * up0 * up1;
         if constexpr (L::kIntegerKeys) {
 #pragma unroll
           for (int part = 0; part < kPer; ++part) {
             // three balanced digits of base 128
-            const int n = __float2int_rn(value[step][b][part] * up0 * up1);
+            const int n = __float2int_rn(x[part]);
             const int d0 = ((n + 64) & 127) - 64, n1 = (n - d0) >> 7, d1 = ((n1 + 64) & 127) - 64, d2 = (n1 - d1) >> 7;
             term[0][b] |= (static_cast<uint32_t>(d0) & 255U) << (8 * part);
             term[1][b] |= (static_cast<uint32_t>(d1) & 255U) << (8 * part);
             term[2][b] |= (static_cast<uint32_t>(d2) & 255U) << (8 * part);
           }
         } else {
-          const float x0 = value[step][b][0] * up0 * up1, x1 = value[step][b][1] * up0 * up1;
-          term[0][b] = pack_half(x0, x1);
+          term[0][b] = pack_half(x[0], x[1]);
           const float2 f = unpack_half(term[0][b]);
-          term[1][b] = pack_half(x0 - f.x, x1 - f.y);
+          term[1][b] = pack_half(x[0] - f.x, x[1] - f.y);
         }
       }
 #pragma unroll
-      for (int i = 0; i < X::kTerms; ++i) {
-        if constexpr (X::kQueryInRegisters) q[step * X::kTerms + i] = make_uint2(term[i][0], term[i][1]);
-        else if (phase == 0U) fragments[(step * X::kTerms + i) * 32 + lane] = make_uint2(term[i][0], term[i][1]);
+      for (int i = 0; i < 3; ++i) made[i] = make_uint2(term[i][0], term[i][1]);
+    };
+    uint2 q[X::kQueryInRegisters ? X::kSteps * X::kTerms : 1];
+    if constexpr (X::kSharedQuery) {
+      for (int step = static_cast<int>(phase); step < X::kSteps; step += static_cast<int>(phases)) {
+        uint2 made[3];
+        make_terms(step, made);
+#pragma unroll
+        for (int i = 0; i < X::kTerms; ++i) fragments[(step * X::kTerms + i) * 32 + lane] = made[i];
       }
-    }
-    if constexpr (!X::kQueryInRegisters) {
       __syncthreads();
-      w.begin(x, at, first, last, phase, phases, ring);
+      if constexpr (X::kQueryInRegisters) {
+#pragma unroll
+        for (int i = 0; i < X::kSteps * X::kTerms; ++i) q[i] = w.fragments[i * 32 + lane];
+      }
+    } else if constexpr (X::kQueryInRegisters) {
+#pragma unroll
+      for (int step = 0; step < X::kSteps; ++step) {
+        uint2 made[3];
+        make_terms(step, made);
+#pragma unroll
+        for (int i = 0; i < X::kTerms; ++i) q[step * X::kTerms + i] = made[i];
+      }
+    } else {  // the fragments take the queries' place
+      uint2 made[X::kSteps][3];
+#pragma unroll
+      for (int step = 0; step < X::kSteps; ++step) make_terms(step, made[step]);
+      __syncthreads();
+      if (phase == 0U) {
+#pragma unroll
+        for (int step = 0; step < X::kSteps; ++step)
+#pragma unroll
+          for (int i = 0; i < X::kTerms; ++i) fragments[(step * X::kTerms + i) * 32 + lane] = made[step][i];
+      }
+      __syncthreads();
     }
+    if constexpr (!X::kQueryInRegisters) w.begin(x, at, first, last, phase, phases, ring);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       w.run.reference[h] = -INFINITY;
