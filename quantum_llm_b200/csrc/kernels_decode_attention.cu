@@ -24,13 +24,17 @@
 // of keys that a fragment packs are put together by byte permutes.  Key 2 r stands in row r of a 16-key
 // block, key 2 r + 1 in row r + 8, so that a lane's two keys (scales, scores) are neighbours.
 //
-// Numerics: codes of Q8 and Q4H records are small integers, exact in F16; their scales multiply scores and
-// weights in FP32.  A query row is scaled by a power of two to [2^8, 2^9) before it becomes F16, so BF16 rows
-// lose nothing that FP32 sums would keep; FP32 rows become two F16 terms (22 bits), and so do the weights
-// p that meet V.  With 16-bit rows p is one F16 term: 2^-11 of each weight, below the rounding of a BF16 row and
-// equal to that of an F16 row before averaging.  The softmax reference is only moved when p would exceed 2^15 (one
-// vote per tile instead of a reduction) and is set so that the largest p is 2^7 then: F16 holds p down to 2^-32 of
+// Numerics.  Codes of Q8 and Q4H records are small integers: K's meet the query as INT8 (mma.sync m16n8k32), the query as a
+// 21-bit integer relative to the largest of its row in three balanced digits of base 128, so that every product and sum
+// of a digit is exact (one INT8 instruction takes the time of an F16 one of half as many dimensions, and K needs no
+// conversion); V's are exact in F16.  The records' scales multiply scores and weights in FP32.  For an F16 cache the query is
+// scaled by a power of two to [2^8, 2^9) and becomes F16: exact for F16 and (down to 2^-22 of the largest) BF16 rows, two terms
+// (22 bits) for FP32 rows.  The weights p that meet V are two F16 terms with FP32 and F16 rows, and one with BF16 rows: 2^-12 of
+// each weight there, an eighth of the output's own rounding.  The softmax reference is only moved when p would exceed 2^15
+// (one vote per tile instead of a reduction) and is set so that the largest p is 2^7 then: F16 holds p down to 2^-32 of
 // the largest, and a quantised V's scale is counted into the reference so that this holds for p times scale.
+#include <type_traits>
+
 #include "kernels.h"
 #include "kv_batch.cuh"
 #include "launch.cuh"
@@ -255,7 +259,8 @@ struct Cursor {
 
 template <typename T, int ENC, int HD>
 struct Traits {
-  static constexpr bool kPrecise = sizeof(T) == 4;
+  static constexpr bool kPrecise = sizeof(T) == 4;  // two F16 terms for the query,
+  static constexpr bool kPreciseWeights = !std::is_same<T, __nv_bfloat16>::value;  // and for the weights
   // fragments of the query per step: F16 terms, or INT8 digits of a 21-bit integer
   static constexpr int kTerms = Layout<ENC, HD>::kIntegerKeys ? 3 : kPrecise ? 2 : 1;
   static constexpr int kSteps = Layout<ENC, HD>::kSteps;
@@ -484,7 +489,7 @@ struct Warp {
   }
   __device__ __forceinline__ void add_values(const uint32_t (&v)[L::kRegs], const float (&p)[4]) {
     uint32_t hi[2], lo[2] = {0U, 0U};
-    weight_fragments<X::kPrecise>(p, hi, lo);
+    weight_fragments<X::kPreciseWeights>(p, hi, lo);
     // keys 4c, 4c+2 are k = 2c, 2c+1 of the product, keys 4c+1, 4c+3 k = 2c+8, 2c+9
 #pragma unroll
     for (int w = 0; w < HD / 64; ++w) {
@@ -496,7 +501,7 @@ struct Warp {
           const uint32_t a0 = __byte_perm(k0, k2, 0x5410), a1 = __byte_perm(k0, k2, 0x7632);
           const uint32_t a2 = __byte_perm(k1, k3, 0x5410), a3 = __byte_perm(k1, k3, 0x7632);
           mma16816(run.out[4 * w + i], a0, a1, a2, a3, hi[0], hi[1]);
-          if constexpr (X::kPrecise) mma16816(run.out[4 * w + i], a0, a1, a2, a3, lo[0], lo[1]);
+          if constexpr (X::kPreciseWeights) mma16816(run.out[4 * w + i], a0, a1, a2, a3, lo[0], lo[1]);
         }
       } else {
         const uint32_t k0 = v[w], k1 = v[HD / 64 + w], k2 = v[2 * (HD / 64) + w], k3 = v[3 * (HD / 64) + w];
@@ -510,7 +515,7 @@ struct Warp {
           for (int i = 0; i < 2; ++i) {
             const int mt = 4 * w + 2 * half + i;
             mma16816(run.out[mt], even[2 * i], even[2 * i + 1], odd[2 * i], odd[2 * i + 1], hi[0], hi[1]);
-            if constexpr (X::kPrecise) mma16816(run.out[mt], even[2 * i], even[2 * i + 1], odd[2 * i], odd[2 * i + 1], lo[0], lo[1]);
+            if constexpr (X::kPreciseWeights) mma16816(run.out[mt], even[2 * i], even[2 * i + 1], odd[2 * i], odd[2 * i + 1], lo[0], lo[1]);
           }
         }
       }
@@ -774,7 +779,7 @@ struct Warp {
     if (scores) put_scores(scores, capacity, heads_here, token, last, s[0]);
     softmax_tile<HD, 1, true>(run, s, vs);
     uint32_t hi[2], lo[2] = {0U, 0U};
-    weight_fragments<X::kPrecise>(s[0], hi, lo);
+    weight_fragments<X::kPreciseWeights>(s[0], hi, lo);
     uint32_t v[4][HD / 32];
 #pragma unroll
     for (uint32_t k = 0; k < 4U; ++k) {
@@ -790,7 +795,7 @@ struct Warp {
         const uint32_t even = __byte_perm(v[0][j], v[2][j], selector), odd = __byte_perm(v[1][j], v[3][j], selector);
         const uint32_t a0 = bytes_to_half(even), a1 = bytes_to_half(even >> 8U), a2 = bytes_to_half(odd), a3 = bytes_to_half(odd >> 8U);
         mma16816(run.out[2 * j + half], a0, a1, a2, a3, hi[0], hi[1]);
-        if constexpr (X::kPrecise) mma16816(run.out[2 * j + half], a0, a1, a2, a3, lo[0], lo[1]);
+        if constexpr (X::kPreciseWeights) mma16816(run.out[2 * j + half], a0, a1, a2, a3, lo[0], lo[1]);
       }
   }
 };

@@ -24,7 +24,7 @@ namespace qllm {
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kWarpsWanted = 4096;  // of a launch
+constexpr uint32_t kWarpsWanted = 2048;  // of a launch (rows of 40 + 16 heads of 128: 2048: 9.4, 4096: 10.9, 8192: 12.9 us for 1024 rows)
 
 template <int kLanes>
 __device__ __forceinline__ float head_sum(float v) {
@@ -72,6 +72,11 @@ __device__ __forceinline__ void copy16(void* to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
 }
 
+template <typename T>
+__host__ __device__ constexpr uint32_t stages() {
+  return sizeof(T) == 2U ? 4U : 2U;  // 32 KiB of a block, of which four share a multiprocessor (three for FP32: no faster)
+}
+
 // One warp per task: `passes` times kHeadsPerWarp heads of one row.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 4)
@@ -80,10 +85,11 @@ norm_rope_store_kernel(const __grid_constant__ NormRopeStoreArgs a, uint32_t tas
   constexpr uint32_t kLanes = kActive == 12U ? 16U : kActive;  // lanes set aside for it
   constexpr uint32_t kHeadsPerWarp = 32U / kLanes;
   constexpr uint32_t kTurns = kLanes / 4U;                     // cosines a lane works out
-  constexpr uint32_t kStages = sizeof(T) == 2U ? 4U : 2U;      // passes in flight: 32 KiB of a block
+  constexpr uint32_t kStages = stages<T>();                    // passes in flight
   constexpr uint32_t kWords = sizeof(T) / 2U;                  // 16-byte words of eight values
   __shared__ alignas(16) float norm[2][HD];
-  __shared__ uint4 ring[kStages][2U * kWords][kThreads];       // a lane's values of the passes to come; nobody else reads them
+  extern __shared__ uint4 ring_memory[];                       // a lane's values of the passes to come; nobody else reads them
+  uint4 (&ring)[kStages][2U * kWords][kThreads] = *reinterpret_cast<uint4 (*)[kStages][2U * kWords][kThreads]>(ring_memory);
   for (uint32_t i = threadIdx.x; i < 2U * HD; i += kThreads) norm[i / HD][i % HD] = (i < HD ? a.q_norm : a.k_norm)[i % HD];
   __syncthreads();
   const uint64_t task = static_cast<uint64_t>(blockIdx.x) * (kThreads / 32U) + (threadIdx.x >> 5U);
@@ -228,8 +234,9 @@ int launch(const NormRopeStoreArgs& a, cudaStream_t stream) {
   const uint32_t tasks = (all + passes - 1U) / passes;
   const uint64_t blocks = (static_cast<uint64_t>(tasks) * a.rows + kThreads / 32U - 1U) / (kThreads / 32U);
   if (blocks > 0x7FFFFFFFULL) return fail(QLLM_INVALID_ARGUMENT, "QK norm / RoPE / KV store: too many rows");
+  constexpr uint32_t kShared = stages<T>() * sizeof(T) * kThreads * 16U;
   count_launch();
-  return check_cuda(launch_ordered(norm_rope_store_kernel<T, HD>, dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, stream, a, tasks, passes),
+  return check_cuda(launch_ordered(norm_rope_store_kernel<T, HD>, dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), kShared, stream, a, tasks, passes),
                     "qk_norm_rope_store");
 }
 
