@@ -348,16 +348,58 @@ kv_select_kernel(const __grid_constant__ KvEvictArgs a, RowHeader* headers, uint
   if (rank == blocks - 1U && warp == kSelectWarps - 1U && lane == 0U) headers[row] = {n, m, min(movers, most), 0U};
 }
 
-// Words of one record, K and V: 16 bytes each (F16, Q4H and its 2-byte scale), or 4 (Q8, whose records are on
-// 2-byte boundaries) and the two bytes left.
+// Words of 16 bytes of one record, K and V, and the 2-byte scales of Q4H.
 __host__ __device__ __forceinline__ uint32_t record_words(uint32_t encoding, uint32_t hd) {
-  return 2U * (encoding == QLLM_KV_F16 ? hd / 8U : encoding == QLLM_KV_Q4H ? hd / 32U + 1U : hd / 4U + 1U);
+  return 2U * (encoding == QLLM_KV_F16 ? hd / 8U : hd / 32U + 1U);
+}
+
+// Q8 records are on 2-byte boundaries: a warp copies whole records, K and V, in words of four bytes from the target's first
+// 4-byte boundary on, and the two bytes before or behind them.  codes[0], [1]: K records of targets and sources.
+template <uint32_t HD>
+__device__ __forceinline__ void move_q8(uint8_t* const (&codes)[2][kMoveBatch], uint32_t count, size_t to_value) {
+  constexpr uint32_t kEach = HD / 64U;         // words of a lane, K and V together
+  constexpr uint32_t kMoves = HD <= 128U ? 4U : 2U;
+  const uint32_t lane = threadIdx.x & 31U, warp = threadIdx.x >> 5U;
+  for (uint32_t j0 = warp * kMoves; j0 < count; j0 += kMoveThreads / 32U * kMoves) {
+    uint32_t data[kMoves][kEach];
+    uint16_t rest[kMoves];
+    uint8_t* to[kMoves];
+#pragma unroll
+    for (uint32_t m = 0; m < kMoves; ++m) {
+      to[m] = nullptr;
+      rest[m] = 0U;
+      if (j0 + m >= count || !codes[0][j0 + m] || !codes[1][j0 + m]) continue;
+      to[m] = codes[0][j0 + m];
+      const uint8_t* from = codes[1][j0 + m];
+      const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to[m])) & 2U;
+      const bool same = ((reinterpret_cast<uintptr_t>(to[m]) ^ reinterpret_cast<uintptr_t>(from)) & 2U) == 0U;
+#pragma unroll
+      for (uint32_t u = 0; u < kEach; ++u) {
+        const uint32_t i = lane + 32U * u;
+        const uint8_t* p = from + (i >= HD / 4U ? to_value : 0U) + odd + 4U * (i % (HD / 4U));
+        data[m][u] = same ? *reinterpret_cast<const uint32_t*>(p)
+                          : *reinterpret_cast<const uint16_t*>(p) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + 2)) << 16U;
+      }
+      if (lane < 2U) rest[m] = *reinterpret_cast<const uint16_t*>(from + (lane ? to_value : 0U) + (odd ? 0U : HD));
+    }
+#pragma unroll
+    for (uint32_t m = 0; m < kMoves; ++m) {
+      if (!to[m]) continue;
+      const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to[m])) & 2U;
+#pragma unroll
+      for (uint32_t u = 0; u < kEach; ++u) {
+        const uint32_t i = lane + 32U * u;
+        *reinterpret_cast<uint32_t*>(to[m] + (i >= HD / 4U ? to_value : 0U) + odd + 4U * (i % (HD / 4U))) = data[m][u];
+      }
+      if (lane < 2U) *reinterpret_cast<uint16_t*>(to[m] + (lane ? to_value : 0U) + (odd ? 0U : HD)) = rest[m];
+    }
+  }
 }
 
 // Moves in batches: first a thread per move finds its two pages and moves weight and position, then all threads copy
 // words, kAtOnce of them in flight each.  The batches of all rows stand in one line, of which each block takes an equal
 // share: rows that move nothing cost no blocks (empty ones took 8 us of 32 for 192 rows).
-template <uint32_t ENC>
+template <uint32_t ENC, uint32_t HD>
 __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_constant__ KvEvictArgs a, const RowHeader* headers,
                                                                const uint2* pairs, uint32_t most) {
   constexpr int kAtOnce = 4;
@@ -406,15 +448,16 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_cons
   __syncthreads();
   uint32_t row = start_row;
   unsigned long long base = start_base;
-  const uint32_t pt = a.cache.page_tokens, hd = a.cache.head_dim;
+  constexpr uint32_t hd = HD;
+  const uint32_t pt = a.cache.page_tokens;
   const uint32_t words = record_words(ENC, hd), at_once = kMoveThreads / words;  // moves of a block side by side
   const uint32_t local = threadIdx.x / words, part = threadIdx.x % words;
   const bool value = part >= words / 2U;
   const uint32_t word = value ? part - words / 2U : part;
   const bool is_scale = ENC == QLLM_KV_Q4H && word == hd / 32U;
   // from a record's K codes (scale) to the thread's word
-  const size_t to_value = value ? kv_codes_at(a.cache, true, 0U, 0U) : 0U;
-  const size_t delta = to_value + (ENC == QLLM_KV_Q8 || is_scale ? 0U : 16U * word);
+  const size_t to_value = kv_codes_at(a.cache, true, 0U, 0U);
+  const size_t delta = (value ? to_value : 0U) + (is_scale ? 0U : 16U * word);
   for (; batch < end; ++batch) {
     uint32_t moves = headers[row].moves;
     while (batch - base >= (moves + kMoveBatch - 1U) / kMoveBatch) {
@@ -444,6 +487,10 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_cons
       }
     }
     __syncthreads();
+    if constexpr (ENC == QLLM_KV_Q8) {
+      move_q8<HD>(codes, count, to_value);
+      continue;
+    }
     if (local >= at_once) continue;
     for (uint32_t j0 = local; j0 < count; j0 += kAtOnce * at_once) {
       uint8_t* to[kAtOnce];
@@ -454,20 +501,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_cons
         to[u] = nullptr;
         data[u] = make_uint4(0U, 0U, 0U, 0U);
         if (j >= count || !codes[0][j] || !codes[1][j]) continue;
-        if constexpr (ENC == QLLM_KV_Q8) {
-          // hd + 2 bytes: whole words from the target's first 4-byte boundary on, and the two bytes before or behind them
-          to[u] = codes[0][j] + delta;
-          const uint8_t* from = codes[1][j] + delta;
-          const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to[u])) & 2U;
-          const uint32_t offset = word < hd / 4U ? odd + 4U * word : odd ? 0U : hd;
-          to[u] += offset;
-          const uint8_t* p = from + offset;
-          if (word < hd / 4U && (reinterpret_cast<uintptr_t>(p) & 2U) == 0U) data[u].x = *reinterpret_cast<const uint32_t*>(p);
-          else {
-            data[u].x = *reinterpret_cast<const uint16_t*>(p);
-            if (word < hd / 4U) data[u].x |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + 2)) << 16U;
-          }
-        } else if (is_scale) {
+        if (is_scale) {
           to[u] = scales[0][ENC == QLLM_KV_Q4H ? j : 0U] + delta;
           data[u].x = *reinterpret_cast<const uint16_t*>(scales[1][ENC == QLLM_KV_Q4H ? j : 0U] + delta);
         } else {
@@ -478,8 +512,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_cons
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
         if (!to[u]) continue;
-        if (ENC == QLLM_KV_Q8 ? word == hd / 4U : is_scale) *reinterpret_cast<uint16_t*>(to[u]) = static_cast<uint16_t>(data[u].x);
-        else if (ENC == QLLM_KV_Q8) *reinterpret_cast<uint32_t*>(to[u]) = data[u].x;
+        if (is_scale) *reinterpret_cast<uint16_t*>(to[u]) = static_cast<uint16_t>(data[u].x);
         else *reinterpret_cast<uint4*>(to[u]) = data[u];
       }
     }
@@ -533,9 +566,27 @@ int launch_kv_evict(const KvEvictArgs& a, cudaStream_t stream) {
   const uint64_t batches = static_cast<uint64_t>(rows) * ((most + kMoveBatch - 1U) / kMoveBatch);
   const dim3 grid(static_cast<uint32_t>(max(static_cast<uint64_t>(1U), min(batches, static_cast<uint64_t>(kMoveBlocks) * sms)))), block(kMoveThreads);
   count_launch();
-  if (a.cache.encoding == QLLM_KV_F16) e = launch_pdl(kv_move_kernel<QLLM_KV_F16>, grid, block, 0, stream, a, headers, pairs, most);
-  else if (a.cache.encoding == QLLM_KV_Q4H) e = launch_pdl(kv_move_kernel<QLLM_KV_Q4H>, grid, block, 0, stream, a, headers, pairs, most);
-  else e = launch_pdl(kv_move_kernel<QLLM_KV_Q8>, grid, block, 0, stream, a, headers, pairs, most);
+  const auto move = [&](auto kernel) { return launch_pdl(kernel, grid, block, 0, stream, a, headers, pairs, most); };
+  const uint32_t hd = a.cache.head_dim;
+  switch (a.cache.encoding) {
+    case QLLM_KV_F16:
+      e = hd == 64U    ? move(kv_move_kernel<QLLM_KV_F16, 64>)
+          : hd == 128U ? move(kv_move_kernel<QLLM_KV_F16, 128>)
+          : hd == 192U ? move(kv_move_kernel<QLLM_KV_F16, 192>)
+                       : move(kv_move_kernel<QLLM_KV_F16, 256>);
+      break;
+    case QLLM_KV_Q4H:
+      e = hd == 64U    ? move(kv_move_kernel<QLLM_KV_Q4H, 64>)
+          : hd == 128U ? move(kv_move_kernel<QLLM_KV_Q4H, 128>)
+          : hd == 192U ? move(kv_move_kernel<QLLM_KV_Q4H, 192>)
+                       : move(kv_move_kernel<QLLM_KV_Q4H, 256>);
+      break;
+    default:
+      e = hd == 64U    ? move(kv_move_kernel<QLLM_KV_Q8, 64>)
+          : hd == 128U ? move(kv_move_kernel<QLLM_KV_Q8, 128>)
+          : hd == 192U ? move(kv_move_kernel<QLLM_KV_Q8, 192>)
+                       : move(kv_move_kernel<QLLM_KV_Q8, 256>);
+  }
   return check_cuda(e, "kv_evict move");
 }
 
