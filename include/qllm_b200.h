@@ -457,7 +457,8 @@ int qllm_k_attention(uint32_t encoding, const uint8_t* const* page_table, size_t
  * cache is the one of the calls above (same pages, same records), one page table per sequence.
  *
  * All pointers are device memory of the current device unless stated, 4-byte aligned unless a call
- * asks for more; the calls only enqueue on `stream`, allocate nothing, can be captured into a graph,
+ * asks for more (memory that is not the current device's is refused as far as the call can tell from qkv or page_tables);
+ * the calls only enqueue on `stream`, allocate nothing, can be captured into a graph,
  * and keep nothing in the library, so calls on several streams and threads may run at once as long as
  * they share no workspace and no output.  Graphs that share a workspace must not run at once.
  * Results do not depend on scheduling: the same inputs give the same bits on the same GPU model.
@@ -490,7 +491,8 @@ typedef struct qllm_kv_batch {
  * The record of row r goes to slot row_slot[r] of sequence row_sequence[r] (null: sequence r); a
  * sequence or slot outside the cache stores nothing.  row_slot null: no records at all (page_tables may
  * be null).  A row whose slot is QLLM_PADDING_SLOT is left alone: none of its outputs are written.
- * Two rows of one call must not name the same slot (its record would be a mixture of both).
+ * Two rows of one call must not name the same slot (its record would be a mixture of both), nor may the page of a slot
+ * that is written be another sequence's too.
  * slot_positions [sequences, kv_heads, slot_stride] (optional): positions[r] is written for each
  * head of the slot stored, which is what qllm_k_kv_evict reads.
  * Rows and strides in multiples of 16 bytes.  query may be qkv itself, and key its key heads, with the
@@ -525,7 +527,7 @@ int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const
  * the records move in place and as few as possible.  weights_out and positions_out (== the inputs: in
  * place) hold the kept slots' values at t < m, weights_out is zero for m <= t < n (a slot stored there
  * later starts from nothing), everything else is left alone; lengths_out[s] = m (== lengths_in: in
- * place).  Slots on absent pages move no record. */
+ * place).  Slots on absent pages move no record; a page must not be in more than one sequence's table. */
 size_t qllm_k_kv_evict_workspace_bytes(const qllm_kv_batch* cache, uint32_t budget);
 int qllm_k_kv_evict(const qllm_kv_batch* cache, const uint32_t* lengths_in, uint32_t* lengths_out,
                     const uint32_t* next_positions, uint32_t budget, uint32_t recent, uint32_t sinks,

@@ -27,31 +27,44 @@ bool extent_ok(size_t rows, size_t stride) { return stride <= (static_cast<size_
 size_t extent(size_t rows, size_t stride, size_t width) { return (rows - 1U) * stride + width; }
 
 // Geometry of the cache; 0 or the refusal.
-int check_cache(const qllm_kv_batch* c, const char* what) {
-  const std::string who(what);
-  if (!c || !c->sequences || !c->kv_heads) return fail(QLLM_INVALID_ARGUMENT, "invalid " + who + " batch");
+int check_cache(const qllm_kv_batch* c, const char* who) {
+  if (!c || !c->sequences || !c->kv_heads) return fail(QLLM_INVALID_ARGUMENT, std::string("invalid ") + who + " batch");
   if (c->sequences > 65535U || c->kv_heads > 4096U)
-    return fail(QLLM_INVALID_ARGUMENT, who + " takes at most 65535 sequences and 4096 kv heads");
+    return fail(QLLM_INVALID_ARGUMENT, std::string(who) + " takes at most 65535 sequences and 4096 kv heads");
   if (c->head_dim != 64U && c->head_dim != 128U && c->head_dim != 192U && c->head_dim != 256U)
-    return fail(QLLM_INVALID_ARGUMENT, who + " needs head_dim 64, 128, 192 or 256");
+    return fail(QLLM_INVALID_ARGUMENT, std::string(who) + " needs head_dim 64, 128, 192 or 256");
   return 0;
 }
-int check_pages(const qllm_kv_batch* c, const char* what) {
-  const std::string who(what);
+int check_pages(const qllm_kv_batch* c, const char* who) {
   if (!c->page_tables || !aligned(c->page_tables, 8U) || !c->pages_per_sequence || c->encoding > QLLM_KV_Q8)
-    return fail(QLLM_INVALID_ARGUMENT, "invalid " + who + " cache");
+    return fail(QLLM_INVALID_ARGUMENT, std::string("invalid ") + who + " cache");
   if (!c->page_tokens || c->page_tokens % 16U || c->layer_offset % 16U)
-    return fail(QLLM_INVALID_ARGUMENT, who + " needs page_tokens and layer_offset in multiples of 16");
+    return fail(QLLM_INVALID_ARGUMENT, std::string(who) + " needs page_tokens and layer_offset in multiples of 16");
   if (static_cast<uint64_t>(c->pages_per_sequence) * c->page_tokens >= 0x80000000ULL)
-    return fail(QLLM_INVALID_ARGUMENT, who + " takes fewer than 2^31 slots per sequence");
+    return fail(QLLM_INVALID_ARGUMENT, std::string(who) + " takes fewer than 2^31 slots per sequence");
   if (kv_layer_bytes(c->encoding, 1U, c->kv_heads, c->head_dim) * c->page_tokens >= 0x100000000ULL)
-    return fail(QLLM_INVALID_ARGUMENT, who + " takes pages that hold less than 4 GiB of a layer");
+    return fail(QLLM_INVALID_ARGUMENT, std::string(who) + " takes pages that hold less than 4 GiB of a layer");
   return 0;
 }
 
 // Rows that are read or written in 16-byte words.
 bool rows_ok(const void* p, size_t rows, size_t stride, uint32_t type, size_t width) {
   return p && aligned(p, 16U) && stride >= width && stride * row_bytes(type) % 16U == 0U && extent_ok(rows, stride);
+}
+
+// The call's memory has to be the current device's: a host pointer, or another device's memory, would fault in the kernel.
+// One pointer stands for all of a call's (some 0.2 us).
+int check_device(const void* p, const char* what) {
+  cudaPointerAttributes attributes{};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess) e = cudaPointerGetAttributes(&attributes, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // reported here, not by the next call
+    return check_cuda(e, what);
+  }
+  if ((attributes.type == cudaMemoryTypeDevice && attributes.device == device) || attributes.type == cudaMemoryTypeManaged) return 0;
+  return fail(QLLM_INVALID_ARGUMENT, std::string(what) + ": the call's memory is not the current device's");
 }
 
 }  // namespace
@@ -94,6 +107,7 @@ int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, con
   if ((!query_in_place && overlap(query, q_out, qkv, in)) || (key && !key_in_place && overlap(key, k_out, qkv, in)) ||
       (key && !both_in_place && overlap(key, k_out, query, q_out)))
     return fail(QLLM_INVALID_ARGUMENT, "QK norm / RoPE / KV store: rows overlap and are not in place");
+  if ((rc = check_device(qkv, who))) return rc;
   NormRopeStoreArgs a{*cache, row_type, qkv, qkv_stride, rows, q_heads, rotary_dim, q_norm, k_norm, eps, inv_freq, positions,
                       row_sequence, row_slot, query, query_stride, key, key_stride, slot_positions, slot_stride};
   return launch_norm_rope_store(a, static_cast<cudaStream_t>(stream));
@@ -132,6 +146,7 @@ int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const
   }
   if (!aligned(workspace, 16U) || workspace_bytes < decode_attention_workspace_bytes(*cache, q_heads, weights_out != nullptr))
     return fail(QLLM_INVALID_ARGUMENT, "decode attention workspace is too small or not on a 16-byte boundary");
+  if ((rc = check_device(cache->page_tables, who))) return rc;
   DecodeAttentionArgs a{*cache, row_type, query, query_stride, lengths, q_heads, scale, weights_in, weights_out, weights_stride,
                         out, out_stride, workspace};
   return launch_decode_attention(a, static_cast<cudaStream_t>(stream));
@@ -166,6 +181,7 @@ int qllm_k_kv_evict(const qllm_kv_batch* cache, const uint32_t* lengths_in, uint
     return fail(QLLM_INVALID_ARGUMENT, "KV eviction: arrays overlap and are not in place");
   if (!aligned(workspace, 16U) || workspace_bytes < kv_evict_workspace_bytes(*cache, budget))
     return fail(QLLM_INVALID_ARGUMENT, "KV eviction workspace is too small or not on a 16-byte boundary");
+  if ((rc = check_device(cache->page_tables, who))) return rc;
   KvEvictArgs a{*cache, lengths_in, lengths_out, next_positions, budget, recent, sinks, weights_in, weights_out, positions_in,
                 positions_out, stride, workspace};
   return launch_kv_evict(a, static_cast<cudaStream_t>(stream));

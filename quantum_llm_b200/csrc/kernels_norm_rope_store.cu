@@ -143,9 +143,11 @@ norm_rope_store_kernel(const __grid_constant__ NormRopeStoreArgs a, uint32_t tas
     }
   }
   uint8_t* layer = nullptr;
-  if (a.row_slot && sequence < a.cache.sequences && slot < kv_capacity(a.cache))
+  uint32_t place = 0U;
+  if (a.row_slot && sequence < a.cache.sequences && slot < kv_capacity(a.cache)) {
     layer = kv_page(a.cache, sequence, slot / a.cache.page_tokens);
-  const uint32_t place = slot % a.cache.page_tokens;
+    place = slot % a.cache.page_tokens;
+  }
 
   for (uint32_t base = first; base < last; base += kStages * kHeadsPerWarp) {
 #pragma unroll

@@ -5,6 +5,7 @@
 // (runtime/tools/dense_fp4_provider.cpp:11139-11318, 8529-8635, 8681-8852, 11011-11137),
 // re-arranged so that one step is a fixed launch sequence driven by device-resident
 // state: verify -> accept/rollback kernel -> draft passes, with one host read at the end.
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <memory>
@@ -24,7 +25,7 @@ namespace qllm {
 
 namespace {
 thread_local std::string g_error;
-unsigned long long g_launches = 0;
+std::atomic<unsigned long long> g_launches{0};  // calls may come from several threads
 }  // namespace
 
 void set_error(const std::string& message) { g_error = message; }

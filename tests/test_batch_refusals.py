@@ -23,7 +23,8 @@ def cache(**over):
 
 BAD_CACHES = [dict(sequences=0), dict(sequences=65536), dict(kv_heads=0), dict(head_dim=96), dict(head_dim=0), dict(head_dim=512),
               dict(page_tables=None), dict(page_tables=0x1004), dict(pages_per_sequence=0), dict(page_tokens=0), dict(page_tokens=24),
-              dict(encoding=3), dict(layer_offset=8), dict(pages_per_sequence=1 << 25, page_tokens=64)]
+              dict(encoding=3), dict(layer_offset=8), dict(pages_per_sequence=1 << 25, page_tokens=64),
+              dict(pages_per_sequence=1, page_tokens=1 << 22, kv_heads=4), dict(kv_heads=4097)]
 
 
 def store(L, c=None, **over):
@@ -88,6 +89,26 @@ def test_decode_attention(L, bad):
     dict(positions_out=0x400000), dict(stride=255), dict(workspace=None), dict(workspace=0x800008), dict(workspace_bytes=64)])
 def test_kv_evict(L, bad):
     assert trim(L, **bad) == INVALID and L.qllm_last_error()
+
+
+def test_strides_that_cannot_be_addressed(L):
+    far = 1 << 56
+    assert store(L, qkv_stride=far) == INVALID and store(L, query_stride=far) == INVALID and store(L, key_stride=far) == INVALID
+    assert store(L, slot_stride=far) == INVALID and attend(L, query_stride=far) == INVALID and attend(L, out_stride=far) == INVALID
+    assert attend(L, weights_stride=far) == INVALID and trim(L, stride=far) == INVALID
+    # 60000 sequences of 65536 heads
+    many = dict(sequences=60000, kv_heads=1, head_dim=64)
+    assert attend(L, cache(**many), q_heads=65536, query_stride=65536 * 64, out_stride=65536 * 64, out=0x100000 + (1 << 52)) == INVALID
+
+
+def test_valid_arguments_without_a_gpu_are_an_error(L):
+    """The checks pass, and the first question to the device fails: no call works on the CPU instead."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is present")
+    for call in (store, attend, trim):
+        assert call(L) < 0 and call(L) != INVALID and L.qllm_last_error()
+    assert store(L, cache(page_tables=None, pages_per_sequence=0, page_tokens=0), row_slot=None, row_sequence=None, slot_positions=None) != INVALID
 
 
 def test_workspace_sizes_grow_with_the_batch(L):

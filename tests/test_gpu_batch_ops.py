@@ -166,6 +166,64 @@ def test_norm_rope_store_many_rows_and_infinities():
     assert float(v[7, 0, 1]) == 0.0 and bool(v[7, 0].isfinite().all()) and bool(k[6].isfinite().all())
 
 
+def test_norm_rope_store_needs_no_pages_without_slots():
+    """page_tables null and no page geometry: rows are normed and rotated, nothing is stored."""
+    q, kv, hd, rows = 3, 1, 192, 5
+    x = rand((rows, (q + 2 * kv) * hd), 3).to(BF16)
+    w, inv = 1 + 0.1 * rand(hd, 4), inv_freq(64)
+    query = torch.zeros(rows, q * hd, dtype=BF16, device="cuda")
+    bare = bc.ql.KvBatch(None, 0, 1, 0, 0, 0, kv, hd)
+    bc.ql.check(bc.ql.load().qllm_k_qk_norm_rope_store(
+        bare, bc.ql.ROW_BF16, x.data_ptr(), x.stride(0), rows, q, 64, w.data_ptr(), w.data_ptr(), 1e-6, inv.data_ptr(),
+        u32([9, 8, 7, 6, 5]).data_ptr(), None, None, query.data_ptr(), query.stride(0), None, 0, None, 0, bc.stream()))
+    torch.cuda.synchronize()
+    wq, _, size = bc.exact_norm_rope(x, q, kv, hd, 64, w, w, inv, [9, 8, 7, 6, 5])
+    close_norm(query.view(rows, q, hd), wq, size[:, :q], BF16)
+
+
+def test_memory_that_is_not_the_device_s_is_refused():
+    """A page table (rows) in host memory: refused on the host, no kernel runs."""
+    cache = PagedCache(2, 2, 16, F16, 1, 64)
+    host = cache.descriptor()
+    table = cache.tables.cpu()
+    host.page_tables = table.data_ptr()
+    L, n = bc.ql.load(), u32([5, 5])
+    x = rand((2, 4 * 64), 1)
+    out = torch.zeros(2, 128, device="cuda")
+    ws = torch.zeros(1 << 24, dtype=torch.uint8, device="cuda")
+    w, p = torch.zeros(2, 1, 32, device="cuda"), torch.zeros(2, 1, 32, dtype=torch.int32, device="cuda")
+    assert L.qllm_k_decode_attention(host, 0, x.data_ptr(), 256, n.data_ptr(), 2, 0.1, None, None, 0, out.data_ptr(), 128, ws.data_ptr(),
+                                     ws.numel(), bc.stream()) == -4
+    assert L.qllm_k_kv_evict(host, n.data_ptr(), n.data_ptr(), u32([5, 5]).data_ptr(), 4, 0, 0, w.data_ptr(), w.data_ptr(), p.data_ptr(),
+                             p.data_ptr(), 32, ws.data_ptr(), ws.numel(), bc.stream()) == -4
+    y = x.cpu()
+    assert L.qllm_k_qk_norm_rope_store(cache.descriptor(), 0, y.data_ptr(), 256, 2, 2, 0, out.data_ptr(), out.data_ptr(), 1e-6, None, n.data_ptr(),
+                                       None, n.data_ptr(), out.data_ptr(), 128, None, 0, None, 0, bc.stream()) == -4
+    assert b"current device" in L.qllm_last_error()
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("enc", [F16, Q4H, Q8])
+def test_a_page_pointer_off_its_boundary_stands_for_no_page(enc):
+    q, kv, hd, page = 4, 2, 64, 16
+    cache = PagedCache(1, 3, page, enc, kv, hd, seed=2)
+    cache.tables[0, 1] += 8
+    pool = cache.pool.clone()
+    x = rand((1, (q + 2 * kv) * hd), 3)
+    w, inv = torch.ones(hd, device="cuda"), inv_freq(hd)
+    query, out = torch.zeros(1, q * hd, device="cuda"), torch.zeros(1, q * hd, device="cuda")
+    bc.norm_rope_store(cache, x, q, hd, w, w, inv, u32([20]), u32([0]), u32([20]), query)
+    weights = torch.full((1, kv, 48), -3.0, device="cuda")
+    bc.decode_attention(cache, query, u32([40]), q, 0.2, out, None, weights)
+    cache.tables[0, 1] = 0                         # what the oracle takes for absent
+    check_attention(cache, query, [40], q, 0.2, out, None, weights, F32)
+    cache.tables[0, 1] = cache.tables[0, 0] + 4
+    scores, positions, n = rand((1, kv, 48), 4).exp(), torch.arange(48, device="cuda", dtype=torch.int32).expand(1, kv, 48).clone(), u32([16])
+    bc.evict(cache, n, n, u32([16]), 16, 4, 0, scores, scores, positions, positions)
+    torch.cuda.synchronize()
+    assert torch.equal(pool, cache.pool)
+
+
 # ------------------------------------------------------------------------------- attention
 
 def attention_bounds(dtype, n, hd, p, spread, size, want, v_sum):
@@ -537,6 +595,28 @@ def test_evict_with_absent_pages():
         if a // page not in (1, 3) and b // page not in (1, 3):
             want[a] = before[0, b, 0]
     assert torch.equal(cache.records()[0, :, 0], want)
+
+
+def test_evict_on_two_streams():
+    kv, hd, page, n, budget = 2, 64, 16, 2000, 700
+    caches = [PagedCache(3, 128, page, Q8, kv, hd, seed=i) for i in range(2)]
+    sets = [evict_case("plain", 3, kv, 2048, [n] * 3, 40 + i) for i in range(2)]
+    spaces = [bc.evict_workspace(c, budget) for c in caches]
+    outs = [(torch.zeros_like(w), torch.zeros_like(p), u32([0] * 3)) for w, p in sets]
+    before, length = [c.records() for c in caches], u32([n] * 3)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(2):
+        with torch.cuda.stream(streams[i]):
+            bc.evict(caches[i], length, outs[i][2], length, budget, 50, 4, sets[i][0], outs[i][0], sets[i][1], outs[i][1], spaces[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        after = caches[i].records()
+        for s in range(3):
+            for h in range(kv):
+                source, _, _ = bc.exact_evict(sets[i][0][s, h].tolist(), sets[i][1][s, h].tolist(), n, n, budget, 50, 4)
+                at = torch.tensor(source, dtype=torch.long, device="cuda")
+                assert torch.equal(after[s, :budget, h], before[i][s, at, h]) and torch.equal(outs[i][1][s, h, :budget], sets[i][1][s, h][at])
 
 
 # ------------------------------------------------------------------------------ a run together
