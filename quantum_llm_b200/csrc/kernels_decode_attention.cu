@@ -25,7 +25,7 @@
 // block, key 2 r + 1 in row r + 8, so that a lane's two keys (scales, scores) are neighbours.
 //
 // Numerics.  Codes of Q8 and Q4H records are small integers: K's meet the query as INT8 (mma.sync m16n8k32), the query as a
-// 21-bit integer relative to the largest of its row in three balanced digits of base 128, so that every product and sum
+// 23-bit integer relative to the largest of its row in three digits of base 256, so that every product and sum
 // of a digit is exact (one INT8 instruction takes the time of an F16 one of half as many dimensions, and K needs no
 // conversion); V's are exact in F16.  The records' scales multiply scores and weights in FP32.  For an F16 cache the query is
 // scaled by a power of two to [2^8, 2^9) and becomes F16: exact for F16 and (down to 2^-22 of the largest) BF16 rows, two terms
@@ -261,7 +261,7 @@ template <typename T, int ENC, int HD>
 struct Traits {
   static constexpr bool kPrecise = sizeof(T) == 4;  // two F16 terms for the query,
   static constexpr bool kPreciseWeights = !std::is_same<T, __nv_bfloat16>::value;  // and for the weights
-  // fragments of the query per step: F16 terms, or INT8 digits of a 21-bit integer
+  // fragments of the query per step: F16 terms, or INT8 digits of a 23-bit integer
   static constexpr int kTerms = Layout<ENC, HD>::kIntegerKeys ? 3 : kPrecise ? 2 : 1;
   static constexpr int kSteps = Layout<ENC, HD>::kSteps;
   static constexpr bool kQueryInRegisters = HD <= 128;
@@ -457,20 +457,35 @@ struct Warp {
   static __device__ __forceinline__ void join_digits(const int (&d)[3][4], float (&s)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      s[i] = fmaf(static_cast<float>(d[2][i]), 16384.0F, fmaf(static_cast<float>(d[1][i]), 128.0F, static_cast<float>(d[0][i])));
+      s[i] = fmaf(static_cast<float>(d[2][i]), 65536.0F, fmaf(static_cast<float>(d[1][i]), 256.0F, static_cast<float>(d[0][i])));
   }
   template <int kQ>
   __device__ __forceinline__ void score(const uint2 (&q)[kQ], const uint32_t (&k)[L::kRegs], float (&s)[4]) const {
     if constexpr (ENC == QLLM_KV_F16) {
+      // The tensor cores cut their FP32 sums off instead of rounding them: with FP32 rows no more than 64 dimensions go into
+      // one, and the low terms have one of their own (relative error of the output at head_dim 256 and 20000 keys: 2.8e-6
+      // with one sum, 0.6e-6 so).
+      constexpr int kChain = X::kPrecise ? 4 : X::kSteps;
+      float low[4] = {};
       s[0] = s[1] = s[2] = s[3] = 0.0F;
 #pragma unroll
-      for (int step = 0; step < X::kSteps; ++step) {
-        const int i = 2 * step;  // words 4 w, 4 w + 1 and 4 w + 2, 4 w + 3 of a chunk
+      for (int from = 0; from < X::kSteps; from += kChain) {
+        float high[4] = {};
 #pragma unroll
-        for (int term = 0; term < X::kTerms; ++term) {
-          const uint2 f = query(q, step, term);
-          mma16816(s, k[i], k[HD / 8 + i], k[i + 1], k[HD / 8 + i + 1], f.x, f.y);
+        for (int step = from; step < from + kChain; ++step) {
+          const int i = 2 * step;  // words 4 w, 4 w + 1 and 4 w + 2, 4 w + 3 of a chunk
+#pragma unroll
+          for (int term = 0; term < X::kTerms; ++term) {
+            const uint2 f = query(q, step, term);
+            mma16816(term == 0 ? high : low, k[i], k[HD / 8 + i], k[i + 1], k[HD / 8 + i + 1], f.x, f.y);
+          }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] += high[i];
+      }
+      if constexpr (X::kTerms == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] += low[i];
       }
     } else {
       // the even and the odd nibbles of a word as bytes, sixteen times their value
@@ -926,8 +941,8 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 2));
-    // F16: to [2^8, 2^9); INT8 digits: to [2^19, 2^20)
-    const int up = top > 0.0F && top < INFINITY ? (L::kIntegerKeys ? 19 : 8) - ilogbf(top) : 0;
+    // F16: to [2^8, 2^9); INT8 digits: to [2^21, 2^22)
+    const int up = top > 0.0F && top < INFINITY ? (L::kIntegerKeys ? 21 : 8) - ilogbf(top) : 0;
     float unit = ldexpf(a.scale * kLog2e, -up - (ENC == QLLM_KV_Q4H ? 4 : 0));  // of head r; Q4H codes come times sixteen
     if constexpr (L::kIntegerKeys) {
       const uint32_t lanes = __ballot_sync(0xffffffffU, wrong);
@@ -947,9 +962,9 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
         if constexpr (L::kIntegerKeys) {
 #pragma unroll
           for (int part = 0; part < kPer; ++part) {
-            // three balanced digits of base 128
+            // three digits of base 256, -128..127
             const int n = __float2int_rn(x[part]);
-            const int d0 = ((n + 64) & 127) - 64, n1 = (n - d0) >> 7, d1 = ((n1 + 64) & 127) - 64, d2 = (n1 - d1) >> 7;
+            const int d0 = static_cast<int8_t>(n), n1 = (n - d0) >> 8, d1 = static_cast<int8_t>(n1), d2 = (n1 - d1) >> 8;
             term[0][b] |= (static_cast<uint32_t>(d0) & 255U) << (8 * part);
             term[1][b] |= (static_cast<uint32_t>(d1) & 255U) << (8 * part);
             term[2][b] |= (static_cast<uint32_t>(d2) & 255U) << (8 * part);
