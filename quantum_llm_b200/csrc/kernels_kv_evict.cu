@@ -84,28 +84,52 @@ kv_select_kernel(const __grid_constant__ KvEvictArgs a, RowHeader* headers, uint
   const uint32_t first = min(n, rank * slice), count = min(slice, n - first), quads = (count + 3U) / 4U;
   const bool held = slice <= keys_held;
   bool crowded = false;
-  // The keys, kAhead loads of a thread in flight.  Where the outputs are other arrays, they get what would be there
-  // without a move: the slots below m as they are, zero weights behind.
+  // One key into the histogram `to`, by all lanes of a warp.
+  const auto count_key = [&](uint32_t* to, bool counts_here, uint32_t digit) {
+    const uint32_t who = __ballot_sync(0xffffffffU, counts_here);
+    if (__popc(who) >= 8) {
+      // the digit of the warp's first counting lane is added once for all lanes that share it: equal weights would
+      // otherwise queue up at one address
+      const uint32_t leader = __ffs(who) - 1U;
+      const uint32_t common = __shfl_sync(0xffffffffU, digit, leader);
+      const uint32_t same = __ballot_sync(0xffffffffU, counts_here && digit == common);
+      if (lane == leader) atomicAdd(&to[common], static_cast<uint32_t>(__popc(same)));
+      else if (counts_here && digit != common) atomicAdd(&to[digit], 1U);
+    } else if (counts_here) {
+      atomicAdd(&to[digit], 1U);
+    }
+  };
+  uint32_t buffer = 0U;
+  // The keys, kAhead loads of a thread in flight, and (of keys that are held) the histogram of their first digit while other
+  // warps wait for theirs.  Where the outputs are other arrays, they get what would be there without a move: the slots
+  // below m as they are, zero weights behind.
   const auto make_keys = [&] {
-    for (uint32_t j = tid; j < count; j += kAhead * kSelectThreads) {
+    for (uint32_t j = 0; j < count; j += kAhead * kSelectThreads) {
       float weight[kAhead];
       uint32_t position[kAhead];
 #pragma unroll
       for (uint32_t u = 0; u < kAhead; ++u) {
-        const uint32_t i = j + u * kSelectThreads;
+        const uint32_t i = j + u * kSelectThreads + tid;
         weight[u] = i < count ? w[first + i] : 0.0F;
         position[u] = i < count ? pos[first + i] : 0U;
       }
 #pragma unroll
       for (uint32_t u = 0; u < kAhead; ++u) {
-        const uint32_t i = j + u * kSelectThreads, t = first + i;
+        const uint32_t i = j + u * kSelectThreads + tid, t = first + i;
+        if (j + u * kSelectThreads >= count) break;
+        if (held && n > m) {
+          const uint32_t key = keep_key(a, weight[u], position[u], next, crowded);
+          if (i < count) keys[i] = key;
+          count_key(bins[buffer], i < count, key >> 21U);
+        }
         if (i >= count) continue;
-        if (held && n > m) keys[i] = keep_key(a, weight[u], position[u], next, crowded);
         if (w_out != w) w_out[t] = t < m ? weight[u] : 0.0F;
         if (pos_out != pos && t < m) pos_out[t] = position[u];
       }
     }
   };
+  for (uint32_t i = tid; i < kBins; i += kSelectThreads) bins[0][i] = 0U;
+  __syncthreads();
   make_keys();
   if (n == m) {  // everything stays; the whole cluster leaves
     if (rank == 0U && tid == 0U) headers[row] = {n, m, 0U, 0U};
@@ -133,34 +157,19 @@ kv_select_kernel(const __grid_constant__ KvEvictArgs a, RowHeader* headers, uint
 
   // ---- the m-th largest key
   uint32_t threshold = 0U, ties = 0U;  // kept: keys above the threshold, and the first `ties` slots of that key
-  uint32_t left = m, prefix = 0U, shift = 21U, buffer = 0U;
-  for (uint32_t i = tid; i < kBins; i += kSelectThreads) bins[0][i] = 0U;
-  __syncthreads();
+  uint32_t left = m, prefix = 0U, shift = 21U;
   const uint32_t rounds = (quads + kSelectThreads - 1U) / kSelectThreads;
   for (;;) {
     const uint32_t top = shift + (shift == 0U ? 10U : 11U);  // bits from here on are the prefix
     for (uint32_t j = 0; j < rounds; ++j) {
+      if (held && shift == 21U) break;  // counted
       const uint32_t quad = j * kSelectThreads + tid;
       uint32_t four[4] = {0U, 0U, 0U, 0U};
       if (quad < quads) four_keys(quad, four);
 #pragma unroll
-      for (uint32_t u = 0; u < 4U; ++u) {
-        const uint32_t key = four[u];
-        const bool counts_here = 4U * quad + u < count && (shift == 21U || (key >> top) == prefix);
-        const uint32_t who = __ballot_sync(0xffffffffU, counts_here);
-        const uint32_t digit = (key >> shift) & (shift == 0U ? 1023U : 2047U);
-        if (__popc(who) >= 8) {
-          // the digit of the warp's first counting lane is added once for all lanes that share it: equal weights would
-          // otherwise queue up at one address
-          const uint32_t leader = __ffs(who) - 1U;
-          const uint32_t common = __shfl_sync(0xffffffffU, digit, leader);
-          const uint32_t same = __ballot_sync(0xffffffffU, counts_here && digit == common);
-          if (lane == leader) atomicAdd(&bins[buffer][common], static_cast<uint32_t>(__popc(same)));
-          else if (counts_here && digit != common) atomicAdd(&bins[buffer][digit], 1U);
-        } else if (counts_here) {
-          atomicAdd(&bins[buffer][digit], 1U);
-        }
-      }
+      for (uint32_t u = 0; u < 4U; ++u)
+        count_key(bins[buffer], 4U * quad + u < count && (shift == 21U || (four[u] >> top) == prefix),
+                  (four[u] >> shift) & (shift == 0U ? 1023U : 2047U));
     }
     barrier();
     // thread t: bins 2047 - 4t down to 2044 - 4t of the whole cluster
