@@ -108,6 +108,21 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ void add_scaled(float4& to, const float4& x, float f) {
+  to.x = fmaf(x.x, f, to.x);
+  to.y = fmaf(x.y, f, to.y);
+  to.z = fmaf(x.z, f, to.z);
+  to.w = fmaf(x.w, f, to.w);
+}
+// out / sum to four elements of a row; zeros where no key counts.
+template <typename T>
+__device__ __forceinline__ void put_four(T* to, const float4& out, float sum) {
+  const float scale = sum == 0.0F ? 0.0F : 1.0F / sum;
+  put_row(to, out.x * scale);
+  put_row(to + 1, out.y * scale);
+  put_row(to + 2, out.z * scale);
+  put_row(to + 3, out.w * scale);
+}
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -1048,27 +1063,38 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
           make_uint2(blockIdx.x, static_cast<uint32_t>(((last_unit + 1ULL) * blocks - 1ULL) / total));
     }
     float* place = plan.partials + (static_cast<size_t>(blockIdx.x) * 2U + (begins ? 1U : 0U)) * plan.place;
+    // A thread takes four dimensions of one head, all loads before the first use (one dimension and one warp after the other:
+    // 11.7 us instead of 9.8 us for 1 x 1000, 144 us instead of 136 us for 96 ragged sequences).
     for (uint32_t h = 0; h < plan.heads; ++h)
-      for (uint32_t e = threadIdx.x; e < heads_here * HD; e += kThreads) {
-        const uint32_t d = e % HD, g = e / HD;
-        float top = -INFINITY;
-        for (uint32_t p = 0; p < phases; ++p) top = fmaxf(top, merge_max[(p * plan.heads + h) * kHeads + g]);
-        const float reference = top == -INFINITY ? 0.0F : top;
-        float sum = 0.0F, out = 0.0F;
-        for (uint32_t p = 0; p < phases; ++p) {
+      for (uint32_t e = threadIdx.x; e < heads_here * (HD / 4U); e += kThreads) {
+        const uint32_t d = 4U * (e % (HD / 4U)), g = e / (HD / 4U);
+        float tops[kWarps], sums[kWarps], top = -INFINITY;
+        float4 outs[kWarps];
+#pragma unroll
+        for (uint32_t p = 0; p < kWarps; ++p) {
           const uint32_t row = (p * plan.heads + h) * kHeads + g;
-          const float f = exp2_fast(merge_max[row] - reference);
-          sum = fmaf(merge_sum[row], f, sum);  // 0 where no key counts, NaN where a score was NaN
-          out = fmaf(merge_out[row * X::kRow + d], f, out);
+          const bool there = p < phases;
+          tops[p] = there ? merge_max[row] : -INFINITY;
+          sums[p] = there ? merge_sum[row] : 0.0F;
+          outs[p] = there ? *reinterpret_cast<const float4*>(merge_out + row * X::kRow + d) : make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+          top = fmaxf(top, tops[p]);
+        }
+        const float reference = top == -INFINITY ? 0.0F : top;
+        float sum = 0.0F;
+        float4 out = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+#pragma unroll
+        for (uint32_t p = 0; p < kWarps; ++p) {
+          const float f = exp2_fast(tops[p] - reference);
+          sum = fmaf(sums[p], f, sum);  // 0 where no key counts, NaN where a score was NaN
+          add_scaled(out, outs[p], f);
         }
         const uint32_t head = (set * plan.heads + h) * plan.group + tile * kHeads + g;
         if (whole) {
-          put_row(static_cast<T*>(a.out) + static_cast<size_t>(s) * a.out_stride + static_cast<size_t>(head) * HD + d,
-                  sum == 0.0F ? 0.0F : out / sum);
+          put_four(static_cast<T*>(a.out) + static_cast<size_t>(s) * a.out_stride + static_cast<size_t>(head) * HD + d, out, sum);
           if (plan.lse && d == 0U) plan.lse[static_cast<size_t>(s) * a.q_heads + head] = sum == 0.0F ? 0.0F : reference + log2f(sum);
         } else {
           const uint32_t row = h * kHeads + g;
-          place[2U * plan.rows + row * HD + d] = out;
+          *reinterpret_cast<float4*>(place + 2U * plan.rows + row * HD + d) = out;
           if (d == 0U) {
             place[row] = top;
             place[plan.rows + row] = sum;
@@ -1103,39 +1129,40 @@ __device__ __forceinline__ void join_head(const DecodeAttentionArgs& a, const Pl
   __shared__ float4 part[kWays > 1U ? kWays : 1U][kWays > 1U ? HD / 4 : 1];
   T* out = static_cast<T*>(a.out) + static_cast<size_t>(s) * a.out_stride + static_cast<size_t>(head) * HD;
   const uint32_t lane = threadIdx.x & 31U;
+  const uint32_t kv_head = head / plan.group, g = head % plan.group;
+  const uint2 span = span_of(plan, s, kv_head, g);  // together with the length; of no meaning where that is zero
   if (a.lengths[s] == 0U) {
     for (uint32_t d = way * 32U + lane; d < HD; d += 32U * kWays) put_row(out + d, 0.0F);
     return;
   }
-  const uint32_t kv_head = head / plan.group, g = head % plan.group;
-  const uint2 span = span_of(plan, s, kv_head, g);
   const uint32_t count = span.y - span.x + 1U;
   if (count <= 1U) return;
   const uint32_t row = (kv_head % plan.heads) * kHeads + g % kHeads;
-  const float top = top_of(plan, span, row, lane);
+  // lane i has maximum and sum of part i0 + i, those of the first 32 parts from here on
+  float of_part = lane < count ? place_of(plan, span, lane)[row] : -INFINITY;
+  float sum_of_part = lane < count ? place_of(plan, span, lane)[plan.rows + row] : 0.0F;
+  const float top = count <= 32U ? warp_max(of_part) : top_of(plan, span, row, lane);
   const float reference = top == -INFINITY ? 0.0F : top;
   float sum = 0.0F;
   float4 acc[kVectors];
 #pragma unroll
   for (uint32_t v = 0; v < kVectors; ++v) acc[v] = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-  for (uint32_t i0 = 0; i0 < count; i0 += 32U) {  // 32 parts: lane i has the factor of part i0 + i, each warp adds its own
-    const bool there = i0 + lane < count;
-    const float factor = there ? exp2_fast(place_of(plan, span, i0 + lane)[row] - reference) : 0.0F;
-    sum += there ? place_of(plan, span, i0 + lane)[plan.rows + row] * factor : 0.0F;
+  for (uint32_t i0 = 0; i0 < count; i0 += 32U) {  // each warp adds its own parts
+    if (i0) {
+      const bool there = i0 + lane < count;
+      of_part = there ? place_of(plan, span, i0 + lane)[row] : -INFINITY;
+      sum_of_part = there ? place_of(plan, span, i0 + lane)[plan.rows + row] : 0.0F;
+    }
+    const float factor = exp2_fast(of_part - reference);
+    sum = fmaf(sum_of_part, factor, sum);
     const uint32_t here = min(32U, count - i0);
 #pragma unroll 8
     for (uint32_t i = way; i < here; i += kWays) {
       const float f = __shfl_sync(0xffffffffU, factor, i);
       const float4* from = reinterpret_cast<const float4*>(place_of(plan, span, i0 + i) + 2U * plan.rows + row * HD);
 #pragma unroll
-      for (uint32_t v = 0; v < kVectors; ++v) {
-        if (lane + 32U * v >= HD / 4) continue;
-        const float4 x = from[lane + 32U * v];
-        acc[v].x = fmaf(x.x, f, acc[v].x);
-        acc[v].y = fmaf(x.y, f, acc[v].y);
-        acc[v].z = fmaf(x.z, f, acc[v].z);
-        acc[v].w = fmaf(x.w, f, acc[v].w);
-      }
+      for (uint32_t v = 0; v < kVectors; ++v)
+        if (lane + 32U * v < HD / 4) add_scaled(acc[v], from[lane + 32U * v], f);
     }
   }
   sum = warp_sum(sum);
@@ -1151,16 +1178,9 @@ __device__ __forceinline__ void join_head(const DecodeAttentionArgs& a, const Pl
       put_row(out + d, sum == 0.0F ? 0.0F : total / sum);
     }
   } else {
-    const float scale = sum == 0.0F ? 0.0F : 1.0F / sum;
 #pragma unroll
-    for (uint32_t v = 0; v < kVectors; ++v) {
-      if (lane + 32U * v >= HD / 4) continue;
-      T* to = out + 4U * (lane + 32U * v);
-      put_row(to, acc[v].x * scale);
-      put_row(to + 1, acc[v].y * scale);
-      put_row(to + 2, acc[v].z * scale);
-      put_row(to + 3, acc[v].w * scale);
-    }
+    for (uint32_t v = 0; v < kVectors; ++v)
+      if (lane + 32U * v < HD / 4) put_four(out + 4U * (lane + 32U * v), acc[v], sum);
   }
 }
 
@@ -1265,7 +1285,8 @@ int launch(const DecodeAttentionArgs& a, const Plan& plan, cudaStream_t stream) 
   rc = check_cuda(launch_ordered(decode_attention_kernel<T, ENC, HD>, dim3(grid), dim3(kThreads), X::kShared, stream, a, plan),
                   "decode_attention");
   if (rc) return rc;
-  // four warps to a query head as long as they find room at once
+  // The first launch does not call for the second early: blocks that wait beside it made 1 x 32768 Q4H 25.2 us instead of 23.6 us.
+  // Four warps to a query head as long as they find room at once.
   const uint32_t heads = a.cache.sequences * a.q_heads;
   const uint32_t ways = heads <= 8U * sms ? kWarps : 1U;
   const uint32_t joins = ways == kWarps ? heads : (heads + kWarps - 1U) / kWarps;
