@@ -294,6 +294,42 @@ struct Traits {
   static constexpr size_t kShared = (kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes) + kQueryBytes * (ENC == QLLM_KV_Q8 ? 4 : 1);
 };
 
+// Largest magnitude, as the bits of a float, of a row that four lanes share (c = 0 .. 3); NaN counts as the largest.
+template <int HD, typename T>
+__device__ __forceinline__ uint32_t row_maximum(const T* row, uint32_t c) {
+  const uint4* from = reinterpret_cast<const uint4*>(row) + c;
+  uint32_t top = 0U;
+#pragma unroll
+  for (int i = 0; i < HD * static_cast<int>(sizeof(T)) / 64; ++i) {
+    const uint4 x = from[4 * i];
+    const uint32_t word[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (uint32_t v : word) {
+      if constexpr (sizeof(T) == 4)
+        top = max(top, v & 0x7FFFFFFFU);
+      else
+        top = __vmaxu2(top, v & 0x7FFF7FFFU);
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    const unsigned short half = static_cast<unsigned short>(max(top & 0xFFFFU, top >> 16U));
+    if constexpr (std::is_same<T, __half>::value) top = __float_as_uint(__half2float(__ushort_as_half(half)));
+    else top = static_cast<uint32_t>(half) << 16U;
+    top &= 0x7FFFFFFFU;
+  }
+  top = max(top, __shfl_xor_sync(0xffffffffU, top, 1));
+  return max(top, __shfl_xor_sync(0xffffffffU, top, 2));
+}
+__device__ __forceinline__ int exponent(float x) {  // of a positive number: x in [2^exponent, 2^(exponent + 1))
+  const bool small = x < 0x1p-126F;
+  return static_cast<int>(__float_as_uint(small ? x * 0x1p24F : x) >> 23U) - (small ? 151 : 127);
+}
+__device__ __forceinline__ float power_of_two(int n) { return __int_as_float((n + 127) << 23); }  // n in [-126, 127]
+// For operands that fit 32 bits most of the time.
+__device__ __forceinline__ unsigned long long divide(unsigned long long a, uint32_t b) {
+  return a >> 32U ? a / b : static_cast<uint32_t>(a) / b;
+}
+
 // State of the online softmax and of the output in one warp: heads 2 c and 2 c + 1 of the lane.
 template <int HD>
 struct Running {
@@ -867,10 +903,10 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
     if (w < warp) before += warp_units[w];
     total += warp_units[w];
   }
-  const unsigned long long blocks = min(static_cast<unsigned long long>(gridDim.x), total);
+  const uint32_t blocks = static_cast<uint32_t>(min(static_cast<unsigned long long>(gridDim.x), total));
   if (blockIdx.x >= blocks) return;
-  unsigned long long u = blockIdx.x * total / blocks;
-  const unsigned long long end = (blockIdx.x + 1ULL) * total / blocks;
+  unsigned long long u = divide(blockIdx.x * total, blocks);
+  const unsigned long long end = divide((blockIdx.x + 1ULL) * total, blocks);
   if (before <= u && u < before + own) {
     uint32_t s = s0;
     unsigned long long base = before;
@@ -909,7 +945,7 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
       ++s;
       continue;
     }
-    const uint32_t item = static_cast<uint32_t>((u - base) / n), local = static_cast<uint32_t>((u - base) % n);
+    const uint32_t item = static_cast<uint32_t>(divide(u - base, n)), local = static_cast<uint32_t>(u - base - static_cast<unsigned long long>(item) * n);
     const uint32_t take = static_cast<uint32_t>(min(static_cast<unsigned long long>(n - local), end - u));
     const uint32_t from = max(local, plan.cost) - plan.cost, upto = max(local + take, plan.cost) - plan.cost;  // units of tokens
     if (from == upto) {  // the share ends before the item's first token
@@ -931,42 +967,35 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
     Cursor at(a.cache, first + 16U * (phase + phases * (L::kStaged ? 0U : lane % W::kN)), 16U * phases * W::kN);
     typename W::Start x;
     __syncthreads();  // the merge area and the queries of the item before have been read
-    // the first keys are on their way while the query is made ready (where it leaves room in the registers)
-    if constexpr (X::kQueryInRegisters) w.begin(x, at, first, last, phase, phases, ring);
-
-    // ---- the query heads as fragments, scaled to [2^8, 2^9)
+    // the query and (where it leaves room in the registers) the first keys are on their way together
     constexpr uint32_t kChunks = kHeads * HD * sizeof(T) / 16U, kRowChunks = HD * sizeof(T) / 16U;
+    const uint32_t queries = static_cast<uint32_t>(__cvta_generic_to_shared(shared));
     for (uint32_t i = threadIdx.x; i < plan.heads * kChunks; i += kThreads) {
       const uint32_t h = i / kChunks, g = i % kChunks / kRowChunks, chunk = i % kRowChunks;
+      const bool there = g < heads_here;
       const T* q = static_cast<const T*>(a.query) + static_cast<size_t>(s) * a.query_stride +
-                   static_cast<size_t>((set * plan.heads + h) * plan.group + tile * kHeads + g) * HD;
-      *reinterpret_cast<uint4*>(shared + h * X::kQueryBytes + g * X::kQueryPitch + 16U * chunk) =
-          g < heads_here ? reinterpret_cast<const uint4*>(q)[chunk] : make_uint4(0U, 0U, 0U, 0U);
+                   static_cast<size_t>((set * plan.heads + h) * plan.group + tile * kHeads + (there ? g : 0U)) * HD;
+      copy16(queries + h * X::kQueryBytes + g * X::kQueryPitch + 16U * chunk, reinterpret_cast<const uint8_t*>(q) + 16U * chunk, there);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if constexpr (X::kQueryInRegisters) w.begin(x, at, first, last, phase, phases, ring);
+
+    // ---- the query heads as fragments, scaled to [2^8, 2^9) or integers
+    asm volatile("cp.async.wait_group %0;" ::"n"(X::kQueryInRegisters && L::kStaged ? L::kStages - 1 : 0) : "memory");
     __syncthreads();
     const T* row = reinterpret_cast<const T*>(shared + in_set * X::kQueryBytes + w.r * X::kQueryPitch);
     constexpr int kPer = L::kPerRegister;
-    float top = 0.0F;
-    bool wrong = false;  // a NaN or an infinity
-#pragma unroll
-    for (int i = 0; i < HD / 4; ++i) {  // the row's values over its four lanes
-      const float x0 = row_value(row[4 * i + w.c]);
-      wrong = wrong || !(fabsf(x0) < INFINITY);
-      top = fmaxf(top, fabsf(x0));
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 2));
+    const uint32_t top_bits = row_maximum<HD>(row, w.c);
+    const bool wrong = top_bits >= 0x7F800000U;  // a NaN or an infinity
     // F16: to [2^8, 2^9); INT8 digits: to [2^21, 2^22)
-    const int up = top > 0.0F && top < INFINITY ? (L::kIntegerKeys ? 21 : 8) - ilogbf(top) : 0;
-    float unit = ldexpf(a.scale * kLog2e, -up - (ENC == QLLM_KV_Q4H ? 4 : 0));  // of head r; Q4H codes come times sixteen
-    if constexpr (L::kIntegerKeys) {
-      const uint32_t lanes = __ballot_sync(0xffffffffU, wrong);
-      if (lanes >> (4U * w.r) & 15U) unit = NAN;  // integers would lose it
-    }
+    const int up = top_bits != 0U && !wrong ? (L::kIntegerKeys ? 21 : 8) - exponent(__uint_as_float(top_bits)) : 0;
+    const int down = -up - (ENC == QLLM_KV_Q4H ? 4 : 0);  // Q4H codes come times sixteen
+    float unit = a.scale * kLog2e * power_of_two(down / 2) * power_of_two(down - down / 2);  // of head r
+    if (L::kIntegerKeys && wrong) unit = NAN;  // integers would lose it
     w.scale[0] = __shfl_sync(0xffffffffU, unit, 8U * w.c);
     w.scale[1] = __shfl_sync(0xffffffffU, unit, 8U * w.c + 4U);
     // two factors: one may not be a float by itself
-    const float up0 = ldexpf(1.0F, up / 2), up1 = ldexpf(1.0F, up - up / 2);
+    const float up0 = power_of_two(up / 2), up1 = power_of_two(up - up / 2);
     const auto make_terms = [&](int step, uint2 (&made)[3]) {
       uint32_t term[3][2] = {};
 #pragma unroll
