@@ -33,6 +33,12 @@
 // each weight there, an eighth of the output's own rounding.  The softmax reference is only moved when p would exceed 2^15
 // (one vote per tile instead of a reduction) and is set so that the largest p is 2^7 then: F16 holds p down to 2^-32 of
 // the largest, and a quantised V's scale is counted into the reference so that this holds for p times scale.
+//
+// Measured on one B200 (copy 6554 GB/s), device time of both launches: 64 sequences of up to 8192 tokens, F16, 32 query and 4 kv
+// heads of 128, BF16 rows: 99 us, 6.2 TB/s of cache, HBM-bound; 7 of up to 20001, F16, 16 heads of 64, FP32 rows, with weights:
+// 54 us, 4.4 TB/s (two terms a query and a weight: instruction issue, then the weights' pass); 96 of up to 4500, Q8, 40 and 8 heads
+// of 128, with weights: 133 us, 3.7 TB/s (unpacking bytes: instruction issue); 1 of 32768, Q4H, 40 and 8 heads of 128: 21.5 us,
+// 1.6 TB/s (a block's share is some 150 tokens a warp: set-up, merge and join are more than half); 1 of 1000, F16: 9.4 us (latency alone).
 #include <type_traits>
 
 #include "kernels.h"

@@ -13,6 +13,11 @@
 // through distributed shared memory, so that a few long rows use the whole GPU.  Latency-bound: 8 bytes a
 // slot are read once; the rest is a chain of some ten block and cluster barriers.
 // Second launch: the moves, HBM-bound.
+//
+// Measured on one B200 (copy 6554 GB/s): 8 sequences of 32768 slots to half, F16, 8 kv heads of 128: 132 us, of which the
+// selection takes 32 (issue: histogram atomics and the rank walks) and the moves 100 (540 MB, 0.83 of the copy rate); 48 of up to
+// 6001 to 4096, Q4H, 4 heads of 128: 24 us (selection 18: its chain of barriers; moves of 66 bytes 6 to 12); one slot of 4097,
+// 8 heads of 128: 11.6 us, latency alone.
 #include <cooperative_groups.h>
 
 #include "kv_batch.cuh"

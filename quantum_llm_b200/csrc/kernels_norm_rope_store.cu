@@ -16,6 +16,10 @@
 // of one: its lanes share the work of the cosines and sines and hand them round by shuffles, so that
 // warps need no barrier, and the values of the next passes are copied into shared memory (each lane its own)
 // while these are worked on.
+//
+// Measured on one B200 (copy 6554 GB/s): 8192 rows of 40 query and 8 kv heads of 128, BF16: 42 us for 235 MB, 0.85 of the copy
+// rate; 517 FP32 rows of 12 and 2 heads of 256: 8.5 us for 16.8 MB, the start of a launch and one chain of loads; 64 rows and one row:
+// 4.1 and 3.6 us, a launch.
 #include "kv_batch.cuh"
 #include "launch.cuh"
 

@@ -697,3 +697,27 @@ def test_streams_decoded_together_with_a_trimmed_cache(enc, dtype, graph):
                 late = set(range(max(0, where[s] + 1 - recent), where[s] + 1)) | set(range(min(sinks, where[s] + 1)))
                 assert late <= set(positions[s, h, :m].tolist())   # the last tokens and the sinks are always there
     assert following.tolist() == [steps, 30 + steps, 39 + steps]
+
+
+@pytest.mark.parametrize("kind", ["ties", "same position"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_rows_that_eight_blocks_do_not_hold(kind, in_place):
+    """More slots than the shared memory of a whole cluster has room for: the keys are worked out again for every pass."""
+    n, budget, hd, page = 400_007, 150_001, 64, 1024
+    cache = PagedCache(1, -(-n // page), page, Q4H, 1, hd, seed=3)
+    slots = cache.capacity
+    w, p = evict_case("ties", 1, 1, slots, [n], 5)
+    if kind == "same position":  # more protected slots than fit
+        p = torch.where(torch.arange(slots, device="cuda") % 2 == 0, n - 1, p).int()
+    w_in, p_in = w.clone(), p.clone()
+    w_out, p_out = (w_in, p_in) if in_place else (torch.full_like(w, -3), torch.full_like(p, -5))
+    lengths_out = u32([0])
+    before = cache.records()
+    bc.evict(cache, u32([n]), lengths_out, u32([n]), budget, 100, 4, w_in, w_out, p_in, p_out)
+    torch.cuda.synchronize()
+    after = cache.records()
+    source, _, _ = bc.exact_evict(w[0, 0].tolist(), p[0, 0].tolist(), n, n, budget, 100, 4)
+    at = torch.tensor(source, dtype=torch.long, device="cuda")
+    assert lengths_out.tolist() == [budget]
+    assert torch.equal(w_out[0, 0, :budget], w[0, 0][at]) and torch.equal(p_out[0, 0, :budget], p[0, 0][at])
+    assert bool((w_out[0, 0, budget:n] == 0).all()) and torch.equal(after[0, :budget, 0], before[0, at, 0])
