@@ -56,6 +56,7 @@ constexpr uint32_t kItemBytes = 96U * 1024U;  // what a block could read in the 
 constexpr uint32_t kMaxBlocks = 768;    // of the first launch; places in the workspace
 constexpr uint32_t kHeads = 8;          // query heads of an item per kv head
 constexpr uint32_t kWeightTokens = 4 * kThreads;
+constexpr size_t kSharedByDefault = 47U * 1024U;  // of a launch without asking for more, beside the static arrays
 // log2: the largest p of a warp stands between 2^kLift (when the reference was set) and 2^kTop < 65504
 constexpr float kLift = 7.0F, kTop = 15.0F;
 constexpr float kLog2e = 1.4426950408889634F;
@@ -1312,9 +1313,11 @@ int launch(const DecodeAttentionArgs& a, const Plan& plan, cudaStream_t stream) 
   uint32_t sms = 0;
   int rc = multiprocessors(&sms);
   if (rc) return rc;
-  rc = check_cuda(cudaFuncSetAttribute(decode_attention_kernel<T, ENC, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(X::kShared)), "decode_attention shared memory opt-in");
-  if (rc) return rc;
+  if constexpr (X::kShared > kSharedByDefault) {
+    rc = check_cuda(cudaFuncSetAttribute(decode_attention_kernel<T, ENC, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(X::kShared)), "decode_attention shared memory opt-in");
+    if (rc) return rc;
+  }
   const uint32_t grid = min(kMaxBlocks, sms * X::kBlocksPerSm);
   count_launch(2U);
   rc = check_cuda(launch_ordered(decode_attention_kernel<T, ENC, HD>, dim3(grid), dim3(kThreads), X::kShared, stream, a, plan),

@@ -36,6 +36,7 @@ constexpr uint32_t kSlotsPerBlock = 4096;  // a row is spread over more blocks o
 constexpr uint32_t kMaxCluster = 8;
 constexpr uint32_t kAhead = 8;
 constexpr uint32_t kMaxKeys = 48U * 1024U;  // of one block in shared memory; longer rows read weights and positions again
+constexpr uint32_t kKeysByDefault = 7U * 1024U;  // that a launch may hold beside the static arrays without asking for more
 constexpr uint32_t kMoveThreads = 256;
 constexpr uint32_t kMoveBatch = 64;       // moves (32: 142 us, 64: 135 us, 128: 136 us for 8 x 8 rows of 8455)
 constexpr uint32_t kMoveBlocks = 5;       // per multiprocessor, all of them at once
@@ -559,8 +560,10 @@ int launch_kv_evict(const KvEvictArgs& a, cudaStream_t stream) {
     cluster *= 2U;
   const uint32_t slice = ((capacity + cluster - 1U) / cluster + 127U) & ~127U;
   const uint32_t keys_held = min(slice, kMaxKeys);
-  e = cudaFuncSetAttribute(kv_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * sizeof(uint32_t));
-  if (e != cudaSuccess) return check_cuda(e, "kv_evict shared memory opt-in");
+  if (keys_held > kKeysByDefault) {
+    e = cudaFuncSetAttribute(kv_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * sizeof(uint32_t));
+    if (e != cudaSuccess) return check_cuda(e, "kv_evict shared memory opt-in");
+  }
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(rows * cluster);
   config.blockDim = dim3(kSelectThreads);
