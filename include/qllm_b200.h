@@ -509,7 +509,8 @@ int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, con
  *   weights_out[s, h, t] = weights_in[s, h, t] + sum of p_t over the query heads of kv head h
  * query, out [sequences, q_heads * head_dim] of row_type, rows and strides in multiples of 16 bytes, not
  * overlapping; scores, softmax statistics and sums are FP32, the result is rounded once.  A sequence of
- * length 0 (or whose slots are all absent, or all score -inf) gives zeros.  weights_out
+ * length 0 (or whose slots are all absent, or all score -inf) gives zeros.  A query head that holds a NaN or an
+ * infinity gives NaN (BF16 and F16 rows over an F16 cache: what the formulas give).  weights_out
  * [sequences, kv_heads, weights_stride] is optional; weights_in null: zeros; weights_in == weights_out: in
  * place; slots at and behind lengths[s] are left alone.  workspace: at least
  * qllm_k_decode_attention_workspace_bytes bytes on a 16-byte boundary, its content does not matter. */

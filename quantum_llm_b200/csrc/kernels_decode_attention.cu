@@ -560,6 +560,21 @@ struct Warp {
       join_digits(d, s);
     }
   }
+  // One tile of V^T times the weights.  With FP32 rows a sum of its own, added by an instruction that rounds: the tensor cores'
+  // sums, cut off a tile at a time, drift (100000 keys: error of the output 2 to 3 times plain FP32's).
+  static __device__ __forceinline__ void add_product(float (&out)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                     const uint32_t (&hi)[2], const uint32_t (&lo)[2]) {
+    if constexpr (X::kPrecise) {
+      float tile[4] = {};
+      mma16816(tile, a0, a1, a2, a3, lo[0], lo[1]);
+      mma16816(tile, a0, a1, a2, a3, hi[0], hi[1]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[i] += tile[i];
+    } else {
+      mma16816(out, a0, a1, a2, a3, hi[0], hi[1]);
+      if constexpr (X::kPreciseWeights) mma16816(out, a0, a1, a2, a3, lo[0], lo[1]);
+    }
+  }
   __device__ __forceinline__ void add_values(const uint32_t (&v)[L::kRegs], const float (&p)[4]) {
     uint32_t hi[2], lo[2] = {0U, 0U};
     weight_fragments<X::kPreciseWeights>(p, hi, lo);
@@ -573,8 +588,7 @@ struct Warp {
           const uint32_t k2 = v[(2 * (HD / 64) + w) * 4 + i], k3 = v[(3 * (HD / 64) + w) * 4 + i];
           const uint32_t a0 = __byte_perm(k0, k2, 0x5410), a1 = __byte_perm(k0, k2, 0x7632);
           const uint32_t a2 = __byte_perm(k1, k3, 0x5410), a3 = __byte_perm(k1, k3, 0x7632);
-          mma16816(run.out[4 * w + i], a0, a1, a2, a3, hi[0], hi[1]);
-          if constexpr (X::kPreciseWeights) mma16816(run.out[4 * w + i], a0, a1, a2, a3, lo[0], lo[1]);
+          add_product(run.out[4 * w + i], a0, a1, a2, a3, hi, lo);
         }
       } else {
         const uint32_t k0 = v[w], k1 = v[HD / 64 + w], k2 = v[2 * (HD / 64) + w], k3 = v[3 * (HD / 64) + w];
@@ -587,8 +601,7 @@ struct Warp {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int mt = 4 * w + 2 * half + i;
-            mma16816(run.out[mt], even[2 * i], even[2 * i + 1], odd[2 * i], odd[2 * i + 1], hi[0], hi[1]);
-            if constexpr (X::kPreciseWeights) mma16816(run.out[mt], even[2 * i], even[2 * i + 1], odd[2 * i], odd[2 * i + 1], lo[0], lo[1]);
+            add_product(run.out[mt], even[2 * i], even[2 * i + 1], odd[2 * i], odd[2 * i + 1], hi, lo);
           }
         }
       }
@@ -867,8 +880,7 @@ struct Warp {
         const uint32_t selector = half ? 0x7632U : 0x5410U;
         const uint32_t even = __byte_perm(v[0][j], v[2][j], selector), odd = __byte_perm(v[1][j], v[3][j], selector);
         const uint32_t a0 = bytes_to_half(even), a1 = bytes_to_half(even >> 8U), a2 = bytes_to_half(odd), a3 = bytes_to_half(odd >> 8U);
-        mma16816(run.out[2 * j + half], a0, a1, a2, a3, hi[0], hi[1]);
-        if constexpr (X::kPreciseWeights) mma16816(run.out[2 * j + half], a0, a1, a2, a3, lo[0], lo[1]);
+        add_product(run.out[2 * j + half], a0, a1, a2, a3, hi, lo);
       }
   }
 };
