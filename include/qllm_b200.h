@@ -513,7 +513,8 @@ int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, con
  * infinity gives NaN (BF16 and F16 rows over an F16 cache: what the formulas give).  weights_out
  * [sequences, kv_heads, weights_stride] is optional; weights_in null: zeros; weights_in == weights_out: in
  * place; slots at and behind lengths[s] are left alone.  workspace: at least
- * qllm_k_decode_attention_workspace_bytes bytes on a 16-byte boundary, its content does not matter. */
+ * qllm_k_decode_attention_workspace_bytes bytes (0: a cache that the call refuses) on a 16-byte boundary, its content does
+ * not matter. */
 size_t qllm_k_decode_attention_workspace_bytes(const qllm_kv_batch* cache, uint32_t q_heads, int weights);
 int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const void* query, size_t query_stride,
                             const uint32_t* lengths, uint32_t q_heads, float scale, const float* weights_in,

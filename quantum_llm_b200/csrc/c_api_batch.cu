@@ -47,6 +47,13 @@ int check_pages(const qllm_kv_batch* c, const char* who) {
   return 0;
 }
 
+// Whether a workspace has a size: a geometry that the calls take, with or without page tables.
+bool has_size(const qllm_kv_batch* c) {
+  return c && c->sequences && c->sequences <= 65535U && c->kv_heads && c->kv_heads <= 4096U && c->encoding <= QLLM_KV_Q8 &&
+         (c->head_dim == 64U || c->head_dim == 128U || c->head_dim == 192U || c->head_dim == 256U) &&
+         static_cast<uint64_t>(c->pages_per_sequence) * c->page_tokens < 0x80000000ULL;
+}
+
 // Rows that are read or written in 16-byte words.
 bool rows_ok(const void* p, size_t rows, size_t stride, uint32_t type, size_t width) {
   return p && aligned(p, 16U) && stride >= width && stride * row_bytes(type) % 16U == 0U && extent_ok(rows, stride);
@@ -114,7 +121,7 @@ int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, con
 }
 
 size_t qllm_k_decode_attention_workspace_bytes(const qllm_kv_batch* cache, uint32_t q_heads, int weights) {
-  if (!cache) return 0U;
+  if (!has_size(cache)) return 0U;
   return decode_attention_workspace_bytes(*cache, q_heads, weights != 0);
 }
 
@@ -153,7 +160,7 @@ int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const
 }
 
 size_t qllm_k_kv_evict_workspace_bytes(const qllm_kv_batch* cache, uint32_t budget) {
-  if (!cache) return 0U;
+  if (!has_size(cache)) return 0U;
   return kv_evict_workspace_bytes(*cache, budget);
 }
 

@@ -1368,7 +1368,6 @@ int dispatch(const DecodeAttentionArgs& a, const Plan& plan, cudaStream_t stream
 }  // namespace
 
 size_t decode_attention_workspace_bytes(const KvBatch& c, uint32_t q_heads, bool weights) {
-  if (!c.kv_heads) return 0U;
   return plan_of(c, q_heads, weights, nullptr).bytes;
 }
 

@@ -123,3 +123,10 @@ def test_workspace_sizes_grow_with_the_batch(L):
     wide = cache(sequences=1024, pages_per_sequence=2048)
     assert L.qllm_k_decode_attention_workspace_bytes(wide, 16, 1) > 1024 * 16 * 2048 * 64 * 4 > 1 << 32
     assert ctypes.sizeof(ql.KvBatch) == 40
+
+
+@pytest.mark.parametrize("bad", [dict(sequences=0), dict(sequences=65536), dict(kv_heads=0), dict(kv_heads=4097), dict(head_dim=0), dict(head_dim=96),
+                                 dict(encoding=3), dict(pages_per_sequence=1 << 25, page_tokens=64)])
+def test_no_workspace_for_a_cache_that_is_refused(L, bad):
+    assert L.qllm_k_decode_attention_workspace_bytes(cache(**bad), 4, 1) == 0 and L.qllm_k_kv_evict_workspace_bytes(cache(**bad), 100) == 0
+    assert L.qllm_k_decode_attention_workspace_bytes(cache(page_tables=None), 4, 1) > 0
