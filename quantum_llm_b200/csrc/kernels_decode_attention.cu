@@ -1186,23 +1186,25 @@ __device__ __forceinline__ void join_head(const DecodeAttentionArgs& a, const Pl
   const uint32_t count = span.y - span.x + 1U;
   if (count <= 1U) return;
   const uint32_t row = (kv_head % plan.heads) * kHeads + g % kHeads;
-  // lane i has maximum and sum of part i0 + i, those of the first 32 parts from here on
-  float of_part = lane < count ? place_of(plan, span, lane)[row] : -INFINITY;
-  float sum_of_part = lane < count ? place_of(plan, span, lane)[plan.rows + row] : 0.0F;
-  const float top = count <= 32U ? warp_max(of_part) : top_of(plan, span, row, lane);
+  // lane i has maximum and sum of parts 32 c + i: of the first 32 kChunks parts all at once, one chunk after the other behind them
+  constexpr uint32_t kChunks = 3;
+  float of_part[kChunks], sum_of_part[kChunks], top = -INFINITY;
+#pragma unroll
+  for (uint32_t c = 0; c < kChunks; ++c) {
+    const bool there = 32U * c + lane < count;
+    of_part[c] = there ? place_of(plan, span, 32U * c + lane)[row] : -INFINITY;
+    sum_of_part[c] = there ? place_of(plan, span, 32U * c + lane)[plan.rows + row] : 0.0F;
+    top = fmaxf(top, of_part[c]);
+  }
+  top = count <= 32U * kChunks ? warp_max(top) : top_of(plan, span, row, lane);
   const float reference = top == -INFINITY ? 0.0F : top;
   float sum = 0.0F;
   float4 acc[kVectors];
 #pragma unroll
   for (uint32_t v = 0; v < kVectors; ++v) acc[v] = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-  for (uint32_t i0 = 0; i0 < count; i0 += 32U) {  // each warp adds its own parts
-    if (i0) {
-      const bool there = i0 + lane < count;
-      of_part = there ? place_of(plan, span, i0 + lane)[row] : -INFINITY;
-      sum_of_part = there ? place_of(plan, span, i0 + lane)[plan.rows + row] : 0.0F;
-    }
-    const float factor = exp2_fast(of_part - reference);
-    sum = fmaf(sum_of_part, factor, sum);
+  const auto add_chunk = [&](uint32_t i0, float of_lane, float sum_of_lane) {  // each warp adds its own parts
+    const float factor = exp2_fast(of_lane - reference);
+    sum = fmaf(sum_of_lane, factor, sum);
     const uint32_t here = min(32U, count - i0);
 #pragma unroll 8
     for (uint32_t i = way; i < here; i += kWays) {
@@ -1212,6 +1214,13 @@ __device__ __forceinline__ void join_head(const DecodeAttentionArgs& a, const Pl
       for (uint32_t v = 0; v < kVectors; ++v)
         if (lane + 32U * v < HD / 4) add_scaled(acc[v], from[lane + 32U * v], f);
     }
+  };
+#pragma unroll
+  for (uint32_t c = 0; c < kChunks; ++c)
+    if (32U * c < count) add_chunk(32U * c, of_part[c], sum_of_part[c]);
+  for (uint32_t i0 = 32U * kChunks; i0 < count; i0 += 32U) {
+    const bool there = i0 + lane < count;
+    add_chunk(i0, there ? place_of(plan, span, i0 + lane)[row] : -INFINITY, there ? place_of(plan, span, i0 + lane)[plan.rows + row] : 0.0F);
   }
   sum = warp_sum(sum);
   if constexpr (kWays > 1U) {
