@@ -25,7 +25,7 @@
 // block, key 2 r + 1 in row r + 8, so that a lane's two keys (scales, scores) are neighbours.
 //
 // Numerics.  Codes of Q8 and Q4H records are small integers: K's meet the query as INT8 (mma.sync m16n8k32), the query as a
-// 23-bit integer relative to the largest of its row in three digits of base 256, so that every product and sum
+// 23-bit integer (24-bit with FP32 rows) relative to the largest of its row in three digits of base 256, so that every product and sum
 // of a digit is exact (one INT8 instruction takes the time of an F16 one of half as many dimensions, and K needs no
 // conversion); V's are exact in F16.  The records' scales multiply scores and weights in FP32.  For an F16 cache the query is
 // scaled by a power of two to [2^8, 2^9) and becomes F16: exact for F16 and (down to 2^-22 of the largest) BF16 rows, two terms
@@ -35,10 +35,10 @@
 // the largest, and a quantised V's scale is counted into the reference so that this holds for p times scale.
 //
 // Measured on one B200 (copy 6554 GB/s), device time of both launches: 64 sequences of up to 8192 tokens, F16, 32 query and 4 kv
-// heads of 128, BF16 rows: 99 us, 6.2 TB/s of cache, HBM-bound; 7 of up to 20001, F16, 16 heads of 64, FP32 rows, with weights:
+// heads of 128, BF16 rows: 100 us, 6.1 TB/s of cache, HBM-bound; 7 of up to 20001, F16, 16 heads of 64, FP32 rows, with weights:
 // 54 us, 4.4 TB/s (two terms a query and a weight: instruction issue, then the weights' pass); 96 of up to 4500, Q8, 40 and 8 heads
-// of 128, with weights: 133 us, 3.7 TB/s (unpacking bytes: instruction issue); 1 of 32768, Q4H, 40 and 8 heads of 128: 21.5 us,
-// 1.6 TB/s (a block's share is some 150 tokens a warp: set-up, merge and join are more than half); 1 of 1000, F16: 9.4 us (latency alone).
+// of 128, with weights: 133 us, 3.7 TB/s (unpacking bytes: instruction issue); 1 of 32768, Q4H, 40 and 8 heads of 128: 21 us,
+// 1.6 TB/s (a block's share is some 150 tokens a warp: set-up, merge and join are more than half); 1 of 1000, F16: 9.5 us (latency alone).
 #include <type_traits>
 
 #include "kernels.h"
@@ -283,7 +283,7 @@ template <typename T, int ENC, int HD>
 struct Traits {
   static constexpr bool kPrecise = sizeof(T) == 4;  // two F16 terms for the query,
   static constexpr bool kPreciseWeights = !std::is_same<T, __nv_bfloat16>::value;  // and for the weights
-  // fragments of the query per step: F16 terms, or INT8 digits of a 23-bit integer
+  // fragments of the query per step: F16 terms, or INT8 digits of an integer
   static constexpr int kTerms = Layout<ENC, HD>::kIntegerKeys ? 3 : kPrecise ? 2 : 1;
   static constexpr int kSteps = Layout<ENC, HD>::kSteps;
   static constexpr bool kQueryInRegisters = HD <= 128;
@@ -1011,6 +1011,12 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
     const int down = -up - (ENC == QLLM_KV_Q4H ? 4 : 0);  // Q4H codes come times sixteen
     float unit = a.scale * kLog2e * power_of_two(down / 2) * power_of_two(down - down / 2);  // of head r
     if (L::kIntegerKeys && wrong) unit = NAN;  // integers would lose it
+    // FP32 rows: stretched to the largest integer that three digits hold, one to two bits more
+    float stretch = 1.0F;
+    if constexpr (L::kIntegerKeys && X::kPrecise) {
+      if (top_bits != 0U && !wrong) stretch = 127.0F * 65536.0F / (__uint_as_float(top_bits) * power_of_two(up / 2) * power_of_two(up - up / 2));
+      unit /= stretch;
+    }
     w.scale[0] = __shfl_sync(0xffffffffU, unit, 8U * w.c);
     w.scale[1] = __shfl_sync(0xffffffffU, unit, 8U * w.c + 4U);
     // two factors: one may not be a float by itself
@@ -1021,7 +1027,7 @@ decode_attention_kernel(const __grid_constant__ DecodeAttentionArgs a, const __g
       for (int b = 0; b < 2; ++b) {
         float x[kPer];
 #pragma unroll
-        for (int part = 0; part < kPer; ++part) x[part] = row_value(row[L::query_dim(step, b, part, w.c, turn)]) * up0 * up1;
+        for (int part = 0; part < kPer; ++part) x[part] = row_value(row[L::query_dim(step, b, part, w.c, turn)]) * up0 * up1 * stretch;
         if constexpr (L::kIntegerKeys) {
 #pragma unroll
           for (int part = 0; part < kPer; ++part) {
