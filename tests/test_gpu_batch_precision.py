@@ -1,0 +1,79 @@
+"""How exact the decode attention over the paged cache is, against its definition in 64 bits: tighter than the worst-case
+bounds of test_gpu_batch_ops.py, at the places where a term, a digit or a rounding sum could go missing unnoticed.
+
+FP32 rows: the error over the norm of the output.  The softmax puts its weight on keys of a score of about the scores'
+variance: 4 nats, 6 in log2 units, for queries of spread 2.  A score of z is off by some eight roundings of e |z|, a weight by
+ln 2 times that and 4 e: 0.69 * 6 * 8 e + 4 e = 2.2e-6, and the sums add less: 3e-6.
+
+16-bit rows: the share of outputs that are not the nearest value of their type.  What was computed is off by an error of r of the norm,
+and a border between two values lies between it and the exact value for |error| / spacing of them: of the elements above a
+quarter of the norm's share (1 / value averages 1.3 there) 0.8 * 1.3 * r / spacing, the spacing relative to the value 2^-7.5 (BF16) and 2^-10.5
+(F16) on average.  F16 rows: a score is one tensor-core sum of up to 16 products that are cut off, each by up to 2 e of
+the sum, 0.69 * 6 * 32 e = 7.9e-6 of a weight: r = 8e-6, a share of 1.2 %.  BF16 rows: weights of 11 bits, off by 2^-10 / sqrt(12) over
+their leading digits' average of 1.44: r = 2e-4, a share of 3.8 %.  Twice that is allowed."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from tests import batch_cache as bc  # noqa: E402
+from tests.batch_cache import F16, Q4H, Q8, PagedCache, u32  # noqa: E402
+
+E = 2.0 ** -24
+F32, BF16, HF16 = torch.float32, torch.bfloat16, torch.float16
+RELATIVE = {F32: 3e-6, HF16: 8e-6, BF16: 2e-4}
+WRONG = {HF16: 0.024, BF16: 0.076}
+
+
+def rand(shape, seed, spread=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(shape, generator=g, device="cuda") * spread
+
+
+def error(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+def wrongly_rounded(got, want):
+    """The share of the elements that are not the nearest value of their type, small ones left out."""
+    counts = want.abs() >= 0.25 * want.norm() / math.sqrt(want.numel())
+    return float((got != want.to(got.dtype))[counts].double().mean())
+
+
+def check(got, want, dtype, extra=0.0):
+    """`extra`: a relative error beside the ones above."""
+    if dtype == F32:
+        assert error(got, want) <= RELATIVE[F32] + extra, error(got, want)
+    else:
+        assert wrongly_rounded(got, want) <= WRONG[dtype] * (1 + extra / RELATIVE[dtype]), wrongly_rounded(got, want)
+
+
+@pytest.mark.parametrize("q,kv,hd,enc,dtype", [(8, 4, 64, Q8, HF16), (8, 1, 64, F16, HF16), (8, 1, 128, Q4H, HF16), (8, 4, 128, Q8, F32),
+                                               (8, 1, 64, F16, F32), (8, 1, 64, Q4H, F32)])
+def test_attention_of_long_items_that_no_block_shares(q, kv, hd, enc, dtype):
+    """As many long sequences as there are blocks, and V of one sign: a sum that drops a part of a rounding with each tile would
+    be off by their number.  All sequences share one sequence's pages, which are only read."""
+    n, sequences, page = 65536, 800, 256
+    cache = PagedCache(1, n // page, page, enc, kv, hd, seed=5)
+    if enc == F16:
+        both = cache.pool.view(HF16).view(-1, 2, page, kv, hd)
+        both[:, 1] = (1.0 + 0.25 * both[:, 1].float()).half()
+    else:
+        m, half = cache.mine(), cache.bytes // 2
+        if enc == Q8:
+            m.view(-1, 2, page * kv, hd + 2)[:, 1, :, :hd] &= 0x3F
+        else:
+            m[:, half:half + page * kv * hd // 2] &= 0x77
+    many = PagedCache.__new__(PagedCache)
+    many.__dict__.update(cache.__dict__)
+    many.sequences, many.tables = sequences, cache.tables.expand(sequences, -1).contiguous()
+    query = rand((sequences, q * hd), 4, 0.05).to(dtype)
+    out = torch.zeros((sequences, q * hd), dtype=dtype, device="cuda")
+    bc.decode_attention(many, query, u32([n] * sequences), q, hd ** -0.5, out)
+    torch.cuda.synchronize()
+    for s in (0, 401, 799):
+        want = bc.exact_attention(cache, 0, n, query[s], q, hd ** -0.5)[0]
+        check(out[s].view(q, hd), want, dtype)
