@@ -29,10 +29,13 @@
 // of a digit is exact (one INT8 instruction takes the time of an F16 one of half as many dimensions, and K needs no
 // conversion); V's are exact in F16.  The records' scales multiply scores and weights in FP32.  For an F16 cache the query is
 // scaled by a power of two to [2^8, 2^9) and becomes F16: exact for F16 and (down to 2^-22 of the largest) BF16 rows, two terms
-// (22 bits) for FP32 rows.  The weights p that meet V are two F16 terms with FP32 and F16 rows, and one with BF16 rows: 2^-11 of
-// each weight at most there, an eighth of the output's own rounding.  The softmax reference is only moved when p would exceed 2^15
-// (one vote per tile instead of a reduction) and is set so that the largest p is 2^7 then: F16 holds p down to 2^-32 of
-// the largest, and a quantised V's scale is counted into the reference so that this holds for p times scale.
+// (22 bits) for FP32 rows.  The weights p that meet V are two terms of 11 bits with FP32 and F16 rows, and one with BF16 rows: off by
+// 2^-11 of each weight at most there, an eighth of the output's own rounding.  Over an F16 cache the terms are TF32 (m16n8k8, F16 values
+// are TF32 values), which holds a weight of any size to that many bits: the keys that make up the output may all be far below
+// the largest weight, where that key's V is near zero (F16 terms: 20 nats below, FP32 rows were off by 0.7 to 1 %, 40 nats
+// below by all; the time of two TF32 terms is 1 to 7 % above that of F16 terms, of one 0 to 1 %).  Over Q8 and Q4H the terms are
+// F16, of p times V's scale: the reference is set so that the largest of those is 2^7 and moved when one would exceed 2^15 (one vote per tile instead
+// of a reduction), F16 holds them down to 2^-32 of the largest, and a key whose V is small has a small scale.
 //
 // Measured on one B200 (copy 6554 GB/s), device time of both launches: 64 sequences of up to 8192 tokens, F16, 32 query and 4 kv
 // heads of 128, BF16 rows: 100 us, 6.1 TB/s of cache, HBM-bound; 7 of up to 20001, F16, 16 heads of 64, FP32 rows, with weights:
@@ -140,6 +143,16 @@ __device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, 
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma1688(float (&d)[4], float a0, float a1, float a2, float a3, uint32_t b0, uint32_t b1) {  // TF32
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(a2)), "r"(__float_as_uint(a3)), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t to_tf32(float v) {
+  uint32_t d;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(d) : "f"(v));
+  return d;
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t d;
@@ -391,7 +404,7 @@ __device__ __forceinline__ void softmax_tile(Running<HD>& run, float (&s)[kN][4]
   }
 }
 
-// Weights of a block as the B operand (keys x heads), one or two F16 terms.
+// Weights of a block as the B operand (keys x heads) of an F16 product, one or two terms.
 template <bool kPrecise>
 __device__ __forceinline__ void weight_fragments(const float (&p)[4], uint32_t (&hi)[2], uint32_t (&lo)[2]) {
 #pragma unroll
@@ -401,6 +414,23 @@ __device__ __forceinline__ void weight_fragments(const float (&p)[4], uint32_t (
     if constexpr (kPrecise) {
       const float2 f = unpack_half(h);
       lo[k] = transpose8(pack_half(p[2 * k] - f.x, p[2 * k + 1] - f.y));
+    }
+  }
+}
+
+// Weights of a block as the B operands of two TF32 products (keys 4c, 4c + 1 and 4c + 2, 4c + 3), one or two terms each.  The
+// two halves of the FP32 words are transposed one after the other.
+template <bool kPrecise>
+__device__ __forceinline__ void weight_fragments_tf32(const float (&p)[4], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const uint32_t x = __float_as_uint(p[2 * k]), y = __float_as_uint(p[2 * k + 1]);
+    const uint32_t low = transpose8(__byte_perm(x, y, 0x5410)), high = transpose8(__byte_perm(x, y, 0x7632));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // key 4c + 2i + k
+      const float w = __uint_as_float(__byte_perm(low, high, i ? 0x7632U : 0x5410U));
+      hi[2 * i + k] = to_tf32(w);
+      if constexpr (kPrecise) lo[2 * i + k] = to_tf32(w - __uint_as_float(hi[2 * i + k]));
     }
   }
 }
@@ -571,19 +601,26 @@ struct Warp {
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] += tile[i];
   }
+  // F16 cache: TF32 holds its values as they are, and weights of any size.
   __device__ __forceinline__ void add_values(const uint32_t (&v)[L::kRegs], const float (&p)[4]) {
-    uint32_t hi[2], lo[2] = {0U, 0U};
-    weight_fragments<X::kPreciseWeights>(p, hi, lo);
-    // keys 4c, 4c+2 are k = 2c, 2c+1 of the product, keys 4c+1, 4c+3 k = 2c+8, 2c+9
+    uint32_t hi[4], lo[4] = {};
+    weight_fragments_tf32<X::kPreciseWeights>(p, hi, lo);
 #pragma unroll
     for (int w = 0; w < HD / 64; ++w)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t k0 = v[w * 4 + i], k1 = v[(HD / 64 + w) * 4 + i];
-        const uint32_t k2 = v[(2 * (HD / 64) + w) * 4 + i], k3 = v[(3 * (HD / 64) + w) * 4 + i];
-        const uint32_t a0 = __byte_perm(k0, k2, 0x5410), a1 = __byte_perm(k0, k2, 0x7632);
-        const uint32_t a2 = __byte_perm(k1, k3, 0x5410), a3 = __byte_perm(k1, k3, 0x7632);
-        add_product(run.out[4 * w + i], a0, a1, a2, a3, hi, lo);
+        float2 f[4];  // dimensions d, d + 1 of keys 4c .. 4c + 3
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = unpack_half(v[(k * (HD / 64) + w) * 4 + i]);
+        float tile[4] = {};
+        if constexpr (X::kPreciseWeights) {
+          mma1688(tile, f[0].x, f[0].y, f[1].x, f[1].y, lo[0], lo[1]);
+          mma1688(tile, f[2].x, f[2].y, f[3].x, f[3].y, lo[2], lo[3]);
+        }
+        mma1688(tile, f[0].x, f[0].y, f[1].x, f[1].y, hi[0], hi[1]);
+        mma1688(tile, f[2].x, f[2].y, f[3].x, f[3].y, hi[2], hi[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) run.out[4 * w + i][j] += tile[j];
       }
   }
   // Q4H: the blocks of a tile share one sum (one each: 1 x 32768 21.8 us instead of 21.3, 64 x 4500 with F16 rows 81.2 instead of 79.5).

@@ -51,6 +51,34 @@ def check(got, want, dtype, extra=0.0):
         assert wrongly_rounded(got, want) <= WRONG[dtype] * (1 + extra / RELATIVE[dtype]), wrongly_rounded(got, want)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, HF16])
+@pytest.mark.parametrize("gap", [10.0, 14.0, 16.0, 20.0, 23.0, 40.0])
+@pytest.mark.parametrize("n", [40, 2048])
+def test_attention_behind_a_key_that_adds_nothing(dtype, gap, n):
+    """An attention sink: one key scores `gap` nats above all others and its V is zero, so that the output is made of weights
+    far below the largest.  An error of that key's score (8 e |z|) is one of every weight."""
+    q, kv, hd, page = 8, 2, 128, 64
+    if dtype == HF16 and gap > 14.0:
+        pytest.skip("the output is below F16's normal values")
+    cache = PagedCache(1, -(-n // page), page, F16, kv, hd, seed=5)
+    both = cache.pool.view(HF16).view(-1, 2, page, kv, hd)
+    if dtype == HF16:
+        both[:, 1] *= 1024.0
+    query = rand((1, q * hd), 4)
+    query[0].view(q, hd)[:, 0] = 8.0
+    both[:, 0, :, :, 0] = 0.0                                # dimension 0 carries the gap alone
+    first = both[int(cache.index[0, 0])]
+    first[0, 0] = 0.0
+    first[0, 0, :, 0] = gap * hd ** 0.5 / 8.0
+    first[1, 0] = 0.0
+    query = query.to(dtype)
+    out = torch.zeros((1, q * hd), dtype=dtype, device="cuda")
+    bc.decode_attention(cache, query, u32([n]), q, hd ** -0.5, out)
+    torch.cuda.synchronize()
+    want = bc.exact_attention(cache, 0, n, query[0], q, hd ** -0.5)[0]
+    check(out[0].view(q, hd), want, dtype, 8 * E * gap)
+
+
 @pytest.mark.parametrize("q,kv,hd,enc,dtype", [(8, 4, 64, Q8, HF16), (8, 1, 64, F16, HF16), (8, 1, 128, Q4H, HF16), (8, 4, 128, Q8, F32),
                                                (8, 1, 64, F16, F32), (8, 1, 64, Q4H, F32)])
 def test_attention_of_long_items_that_no_block_shares(q, kv, hd, enc, dtype):
