@@ -366,7 +366,8 @@ __device__ __forceinline__ void softmax_tile(Running<HD>& run, float (&s)[kN][4]
 #pragma unroll
   for (int b = 0; b < kN; ++b)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) bias[b][k] = kScaled ? __log2f(fmaxf(fabsf(vscale[b][k]), 0x1p-24F)) : 0.0F;
+    for (int k = 0; k < 2; ++k)  // a scale that is infinite or NaN makes the output so, not the reference
+      bias[b][k] = kScaled ? __log2f(fminf(fmaxf(fabsf(vscale[b][k]), 0x1p-24F), 65504.0F)) : 0.0F;
   float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
   for (int b = 0; b < kN; ++b)

@@ -105,3 +105,22 @@ def test_attention_of_long_items_that_no_block_shares(q, kv, hd, enc, dtype):
     for s in (0, 401, 799):
         want = bc.exact_attention(cache, 0, n, query[s], q, hd ** -0.5)[0]
         check(out[s].view(q, hd), want, dtype)
+
+
+@pytest.mark.parametrize("enc", [Q4H, Q8])
+@pytest.mark.parametrize("n", [40, 9000])
+def test_an_infinite_scale_of_a_value_leaves_the_weights(enc, n):
+    """V of one key is infinite: the output is not a number that counts, the weights of the keys are."""
+    q, kv, hd, page = 4, 1, 128, 64
+    cache = PagedCache(1, -(-n // page), page, enc, kv, hd, seed=5)
+    query = rand((1, q * hd), 4, 2.0)
+    want = bc.exact_attention(cache, 0, n, query[0], q, hd ** -0.5)[1].view(kv, q, n).sum(1)
+    at, place, half, records = int(cache.index[0, 0]), 7, cache.bytes // 2, page * kv
+    halves = cache.pool.view(HF16)
+    halves[at, (half + place * (hd + 2) + hd) // 2 if enc == Q8 else (half + records * hd // 2) // 2 + place] = float("inf")
+    out, weights = torch.zeros(1, q * hd, device="cuda"), torch.zeros(1, kv, cache.capacity, device="cuda")
+    bc.decode_attention(cache, query, u32([n]), q, hd ** -0.5, out, None, weights)
+    torch.cuda.synchronize()
+    assert not bool(out.isfinite().any())
+    # a weight: the score's eight roundings of at most e |z| (the largest is below 16 nats), twice, and the sum's
+    assert bool(((weights[0, :, :n].double() - want).abs() <= want * (2 * 8 * 16 * E + 8 * math.sqrt(n) * E) + 1e-37).all())
