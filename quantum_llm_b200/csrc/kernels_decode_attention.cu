@@ -124,14 +124,15 @@ __device__ __forceinline__ void add_scaled(float4& to, const float4& x, float f)
   to.z = fmaf(x.z, f, to.z);
   to.w = fmaf(x.w, f, to.w);
 }
-// out / sum to four elements of a row; zeros where no key counts.
+// out / sum to four elements of a row; zeros where no key counts, whatever its values are (0 times infinity is none).
 template <typename T>
 __device__ __forceinline__ void put_four(T* to, const float4& out, float sum) {
-  const float scale = sum == 0.0F ? 0.0F : 1.0F / sum;
-  put_row(to, out.x * scale);
-  put_row(to + 1, out.y * scale);
-  put_row(to + 2, out.z * scale);
-  put_row(to + 3, out.w * scale);
+  const bool none = sum == 0.0F;
+  const float scale = 1.0F / sum;
+  put_row(to, none ? 0.0F : out.x * scale);
+  put_row(to + 1, none ? 0.0F : out.y * scale);
+  put_row(to + 2, none ? 0.0F : out.z * scale);
+  put_row(to + 3, none ? 0.0F : out.w * scale);
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -572,9 +573,9 @@ struct Warp {
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[i] += high[i];
       }
-      if constexpr (X::kTerms == 2) {
+      if constexpr (X::kTerms == 2) {  // of an infinite key the low terms have either sign
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] += low[i];
+        for (int i = 0; i < 4; ++i) s[i] += fabsf(s[i]) == INFINITY ? 0.0F : low[i];
       }
     } else {
       // the even and the odd nibbles of a word as bytes, sixteen times their value

@@ -124,3 +124,20 @@ def test_an_infinite_scale_of_a_value_leaves_the_weights(enc, n):
     assert not bool(out.isfinite().any())
     # a weight: the score's eight roundings of at most e |z| (the largest is below 16 nats), twice, and the sum's
     assert bool(((weights[0, :, :n].double() - want).abs() <= want * (2 * 8 * 16 * E + 8 * math.sqrt(n) * E) + 1e-37).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [40, 9000])
+def test_keys_that_all_score_minus_infinity_give_zeros(dtype, n):
+    """Whatever their V holds."""
+    q, kv, hd, page = 4, 2, 64, 64
+    cache = PagedCache(1, -(-n // page), page, F16, kv, hd, seed=5)
+    both = cache.pool.view(HF16).view(-1, 2, page, kv, hd)
+    both[:, 0, :, :, 3] = float("-inf")
+    both[:, 1, ::3] = float("nan")
+    query = rand((1, q * hd), 4).abs().add(0.1).to(dtype)
+    out = torch.full((1, q * hd), 7.0, dtype=dtype, device="cuda")
+    weights = torch.full((1, kv, cache.capacity), -3.0, device="cuda")
+    bc.decode_attention(cache, query, u32([n]), q, 0.1, out, None, weights)
+    torch.cuda.synchronize()
+    assert bool((out == 0).all()) and bool((weights[0, :, :n] == 0).all())
