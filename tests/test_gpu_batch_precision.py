@@ -51,6 +51,63 @@ def check(got, want, dtype, extra=0.0):
         assert wrongly_rounded(got, want) <= WRONG[dtype] * (1 + extra / RELATIVE[dtype]), wrongly_rounded(got, want)
 
 
+CASES = [  # q, kv, hd, encoding, page
+    (16, 4, 128, F16, 64), (8, 8, 64, F16, 16), (6, 2, 192, F16, 48), (12, 2, 256, F16, 64),
+    (16, 4, 128, Q4H, 64), (8, 8, 64, Q4H, 16), (6, 2, 192, Q4H, 48), (12, 2, 256, Q4H, 64),
+    (16, 4, 128, Q8, 64), (5, 5, 64, Q8, 16), (6, 2, 192, Q8, 48), (12, 3, 256, Q8, 64)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, HF16])
+@pytest.mark.parametrize("q,kv,hd,enc,page", CASES)
+def test_attention_precision(q, kv, hd, enc, page, dtype):
+    lengths = [1500, 90, 17]
+    cache = PagedCache(len(lengths), -(-1500 // page), page, enc, kv, hd, seed=hd + enc)
+    query = rand((len(lengths), q * hd), 7, 2.0).to(dtype)
+    out = torch.zeros((len(lengths), q * hd), dtype=dtype, device="cuda")
+    bc.decode_attention(cache, query, u32(lengths), q, hd ** -0.5, out)
+    torch.cuda.synchronize()
+    want = torch.stack([bc.exact_attention(cache, s, n, query[s], q, hd ** -0.5)[0] for s, n in enumerate(lengths)])
+    if dtype == F32:
+        for s in range(len(lengths)):
+            check(out[s].view(q, hd), want[s], dtype)
+    else:
+        check(out.view(-1, q, hd), want, dtype)
+
+
+@pytest.mark.parametrize("q,kv,hd,enc,n,dtype", [(8, 1, 64, F16, 70001, F32), (5, 1, 128, Q4H, 40000, F32), (16, 4, 128, Q8, 33333, F32),
+                                                 (8, 1, 128, F16, 50000, BF16), (12, 2, 256, F16, 20000, HF16)])
+def test_attention_precision_of_a_long_sequence(q, kv, hd, enc, n, dtype):
+    cache = PagedCache(1, n // 256 + 1, 256, enc, kv, hd, seed=3)
+    query = rand((1, q * hd), 4, 2.0).to(dtype)
+    out = torch.zeros((1, q * hd), dtype=dtype, device="cuda")
+    bc.decode_attention(cache, query, u32([n]), q, hd ** -0.5, out)
+    torch.cuda.synchronize()
+    check(out[0].view(q, hd), bc.exact_attention(cache, 0, n, query[0], q, hd ** -0.5)[0], dtype)
+
+
+@pytest.mark.parametrize("q,kv,hd,enc,page", CASES)
+def test_a_missing_term_would_show(q, kv, hd, enc, page):
+    """The same comparison with the loss planted in the definition: a query of one term (F16 cache) or two digits (quantised) less
+    than the kernel's, or weights of one F16 term."""
+    n = 1500
+    cache = PagedCache(1, -(-n // page), page, enc, kv, hd, seed=hd + enc)
+    query = rand((1, q * hd), 7, 2.0)
+    want, p, _, _, _ = bc.exact_attention(cache, 0, n, query[0], q, hd ** -0.5)
+    if enc == F16:
+        less = query.half().float()
+    else:
+        unit = query.view(q, hd).abs().amax(-1, keepdim=True) / (127 * 256)
+        less = ((query.view(q, hd) / unit).round() * unit).view(1, -1)
+    got = bc.exact_attention(cache, 0, n, less[0], q, hd ** -0.5)[0]
+    assert error(got.float(), want) > 3e-6
+    group = q // kv
+    _, values, _ = cache.values(0, n)
+    w = (p * (2.0 ** 10 / p.amax(-1, keepdim=True))).half().double()
+    got = torch.einsum("hgt,thd->hgd", (w * p.amax(-1, keepdim=True) / 2.0 ** 10).view(kv, group, n), values).reshape(q, hd)
+    assert error(got.float(), want) > 3e-6
+    assert wrongly_rounded(got.half(), want) > WRONG[HF16]
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, HF16])
 @pytest.mark.parametrize("gap", [10.0, 14.0, 16.0, 20.0, 23.0, 40.0])
 @pytest.mark.parametrize("n", [40, 2048])
