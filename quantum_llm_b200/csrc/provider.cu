@@ -39,16 +39,18 @@ int check_cuda(cudaError_t error, const char* what) {
 }
 int check_launch(const char* what) { return check_cuda(cudaPeekAtLastError(), what); }
 namespace {
-int g_pdl = -1;
+std::atomic<int> g_pdl{-1};  // calls may come from several threads
 }
 bool pdl_enabled() {
-  if (g_pdl < 0) {
+  int on = g_pdl.load(std::memory_order_relaxed);
+  if (on < 0) {
     const char* env = std::getenv("QLLM_PDL");  // QLLM_PDL=0: ordinary launches only
-    g_pdl = (env && env[0] == '0') ? 0 : 1;
+    const int wanted = (env && env[0] == '0') ? 0 : 1;
+    if (g_pdl.compare_exchange_strong(on, wanted, std::memory_order_relaxed)) on = wanted;  // a setting made meanwhile stays
   }
-  return g_pdl == 1;
+  return on == 1;
 }
-void set_pdl_enabled(bool enabled) { g_pdl = enabled ? 1 : 0; }
+void set_pdl_enabled(bool enabled) { g_pdl.store(enabled ? 1 : 0, std::memory_order_relaxed); }
 void count_launch(unsigned launches) { g_launches += launches; }
 unsigned long long launches_counted() { return g_launches; }
 
