@@ -35,9 +35,9 @@ int check_cache(const qllm_kv_batch* c, const char* who) {
     return fail(QLLM_INVALID_ARGUMENT, std::string(who) + " needs head_dim 64, 128, 192 or 256");
   return 0;
 }
-int check_pages(const qllm_kv_batch* c, const char* who) {
-  if (!c->page_tables || !aligned(c->page_tables, 8U) || !c->pages_per_sequence || c->encoding > QLLM_KV_Q8)
-    return fail(QLLM_INVALID_ARGUMENT, std::string("invalid ") + who + " cache");
+// Its pages, but for the table of them.
+int check_page_geometry(const qllm_kv_batch* c, const char* who) {
+  if (!c->pages_per_sequence || c->encoding > QLLM_KV_Q8) return fail(QLLM_INVALID_ARGUMENT, std::string("invalid ") + who + " cache");
   if (!c->page_tokens || c->page_tokens % 16U || c->layer_offset % 16U)
     return fail(QLLM_INVALID_ARGUMENT, std::string(who) + " needs page_tokens and layer_offset in multiples of 16");
   if (static_cast<uint64_t>(c->pages_per_sequence) * c->page_tokens >= 0x80000000ULL)
@@ -47,11 +47,17 @@ int check_pages(const qllm_kv_batch* c, const char* who) {
   return 0;
 }
 
-// Whether a workspace has a size: a geometry that the calls take, with or without page tables.
-bool has_size(const qllm_kv_batch* c) {
-  return c && c->sequences && c->sequences <= 65535U && c->kv_heads && c->kv_heads <= 4096U && c->encoding <= QLLM_KV_Q8 &&
-         (c->head_dim == 64U || c->head_dim == 128U || c->head_dim == 192U || c->head_dim == 256U) &&
-         static_cast<uint64_t>(c->pages_per_sequence) * c->page_tokens < 0x80000000ULL;
+int check_pages(const qllm_kv_batch* c, const char* who) {
+  if (!c->page_tables || !aligned(c->page_tables, 8U)) return fail(QLLM_INVALID_ARGUMENT, std::string("invalid ") + who + " cache");
+  return check_page_geometry(c, who);
+}
+
+// The query heads of an attention batch.
+int check_query_heads(const qllm_kv_batch* c, uint32_t q_heads) {
+  if (!q_heads || q_heads > 65536U || q_heads % c->kv_heads) return fail(QLLM_INVALID_ARGUMENT, "invalid decode attention batch");
+  if (static_cast<uint64_t>(c->sequences) * q_heads > (1U << 28U))
+    return fail(QLLM_INVALID_ARGUMENT, "decode attention takes at most 2^28 query heads over all sequences");
+  return 0;
 }
 
 // Rows that are read or written in 16-byte words.
@@ -121,7 +127,8 @@ int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, con
 }
 
 size_t qllm_k_decode_attention_workspace_bytes(const qllm_kv_batch* cache, uint32_t q_heads, int weights) {
-  if (!has_size(cache)) return 0U;
+  const char* who = "decode attention workspace";
+  if (check_cache(cache, who) || check_page_geometry(cache, who) || check_query_heads(cache, q_heads)) return 0U;
   return decode_attention_workspace_bytes(*cache, q_heads, weights != 0);
 }
 
@@ -131,12 +138,9 @@ int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const
                             size_t workspace_bytes, void* stream) {
   const char* who = "decode attention";
   int rc = check_cache(cache, who);
-  if (rc || (rc = check_pages(cache, who))) return rc;
-  if (!q_heads || q_heads > 65536U || q_heads % cache->kv_heads || row_type > QLLM_ROW_F16 || !lengths || !workspace ||
-      !std::isfinite(scale))
+  if (rc || (rc = check_pages(cache, who)) || (rc = check_query_heads(cache, q_heads))) return rc;
+  if (row_type > QLLM_ROW_F16 || !lengths || !workspace || !std::isfinite(scale))
     return fail(QLLM_INVALID_ARGUMENT, "invalid decode attention batch");
-  if (static_cast<uint64_t>(cache->sequences) * q_heads > (1U << 28U))
-    return fail(QLLM_INVALID_ARGUMENT, "decode attention takes at most 2^28 query heads over all sequences");
   const size_t width = static_cast<size_t>(q_heads) * cache->head_dim, e = row_bytes(row_type);
   if (!rows_ok(query, cache->sequences, query_stride, row_type, width) || !rows_ok(out, cache->sequences, out_stride, row_type, width))
     return fail(QLLM_INVALID_ARGUMENT,
@@ -160,7 +164,8 @@ int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const
 }
 
 size_t qllm_k_kv_evict_workspace_bytes(const qllm_kv_batch* cache, uint32_t budget) {
-  if (!has_size(cache)) return 0U;
+  const char* who = "KV eviction workspace";
+  if (check_cache(cache, who) || check_page_geometry(cache, who)) return 0U;
   return kv_evict_workspace_bytes(*cache, budget);
 }
 

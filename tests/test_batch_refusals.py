@@ -130,3 +130,14 @@ def test_workspace_sizes_grow_with_the_batch(L):
 def test_no_workspace_for_a_cache_that_is_refused(L, bad):
     assert L.qllm_k_decode_attention_workspace_bytes(cache(**bad), 4, 1) == 0 and L.qllm_k_kv_evict_workspace_bytes(cache(**bad), 100) == 0
     assert L.qllm_k_decode_attention_workspace_bytes(cache(page_tables=None), 4, 1) > 0
+
+
+@pytest.mark.parametrize("bad", [b for b in BAD_CACHES if "page_tables" not in b])
+def test_no_workspace_for_any_cache_that_the_calls_refuse(L, bad):
+    assert L.qllm_k_decode_attention_workspace_bytes(cache(**bad), 4, 1) == 0 and L.qllm_last_error()
+    assert L.qllm_k_kv_evict_workspace_bytes(cache(**bad), 100) == 0 and L.qllm_last_error()
+
+
+@pytest.mark.parametrize("q_heads,over", [(0, {}), (5, {}), (65538, {}), (65536, dict(sequences=60000, kv_heads=1))])
+def test_no_workspace_for_query_heads_that_the_attention_refuses(L, q_heads, over):
+    assert L.qllm_k_decode_attention_workspace_bytes(cache(**over), q_heads, 0) == 0 and L.qllm_last_error()
