@@ -18,6 +18,13 @@ bool overlap(const void* p, size_t bytes, const void* q, size_t bytes_q) {
   return a < b + bytes_q && b < a + bytes;
 }
 
+// Lists and arrays of 32-bit elements, null where one is not wanted: the kernels read and write whole words.
+template <typename... P>
+int check_words(const char* who, const P*... p) {
+  if ((aligned(p, 4U) && ...)) return 0;
+  return fail(QLLM_INVALID_ARGUMENT, std::string(who) + " needs lists and arrays on 4-byte boundaries");
+}
+
 size_t row_bytes(uint32_t type) { return type == QLLM_ROW_F32 ? 4U : 2U; }
 
 // Whether `rows` rows `stride` elements apart can be addressed at all.
@@ -97,6 +104,7 @@ int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, con
   if (!rows || !q_heads || q_heads > 65536U || row_type > QLLM_ROW_F16 || !q_norm || !k_norm || !positions ||
       !(eps >= 0.0F) || std::isinf(eps))
     return fail(QLLM_INVALID_ARGUMENT, "invalid QK norm / RoPE / KV store batch");
+  if ((rc = check_words(who, q_norm, k_norm, inv_freq, positions, row_sequence, row_slot, slot_positions))) return rc;
   if (rotary_dim > cache->head_dim || rotary_dim % 16U || (rotary_dim && !inv_freq))
     return fail(QLLM_INVALID_ARGUMENT, "QK norm / RoPE / KV store needs a rotary_dim that is a multiple of 16 and at most head_dim");
   if (row_slot && !row_sequence && rows > cache->sequences)
@@ -141,6 +149,7 @@ int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const
   if (rc || (rc = check_pages(cache, who)) || (rc = check_query_heads(cache, q_heads))) return rc;
   if (row_type > QLLM_ROW_F16 || !lengths || !workspace || !std::isfinite(scale))
     return fail(QLLM_INVALID_ARGUMENT, "invalid decode attention batch");
+  if ((rc = check_words(who, lengths, weights_in, weights_out))) return rc;
   const size_t width = static_cast<size_t>(q_heads) * cache->head_dim, e = row_bytes(row_type);
   if (!rows_ok(query, cache->sequences, query_stride, row_type, width) || !rows_ok(out, cache->sequences, out_stride, row_type, width))
     return fail(QLLM_INVALID_ARGUMENT,
@@ -178,6 +187,7 @@ int qllm_k_kv_evict(const qllm_kv_batch* cache, const uint32_t* lengths_in, uint
   if (rc || (rc = check_pages(cache, who))) return rc;
   if (!lengths_in || !lengths_out || !next_positions || !weights_in || !weights_out || !positions_in || !positions_out || !workspace)
     return fail(QLLM_INVALID_ARGUMENT, "invalid KV eviction batch");
+  if ((rc = check_words(who, lengths_in, lengths_out, next_positions, weights_in, weights_out, positions_in, positions_out))) return rc;
   if (!budget || static_cast<uint64_t>(recent) + sinks > budget)
     return fail(QLLM_INVALID_ARGUMENT, "KV eviction needs a budget that holds the recent tokens and the sinks");
   if (stride < kv_capacity(*cache) || !extent_ok(static_cast<size_t>(cache->sequences) * cache->kv_heads, stride))

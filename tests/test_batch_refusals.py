@@ -141,3 +141,10 @@ def test_no_workspace_for_any_cache_that_the_calls_refuse(L, bad):
 @pytest.mark.parametrize("q_heads,over", [(0, {}), (5, {}), (65538, {}), (65536, dict(sequences=60000, kv_heads=1))])
 def test_no_workspace_for_query_heads_that_the_attention_refuses(L, q_heads, over):
     assert L.qllm_k_decode_attention_workspace_bytes(cache(**over), q_heads, 0) == 0 and L.qllm_last_error()
+
+
+@pytest.mark.parametrize("call,name", [(store, n) for n in ("q_norm", "k_norm", "inv_freq", "positions", "row_sequence", "row_slot", "slot_positions")] +
+                         [(attend, n) for n in ("lengths", "weights_in", "weights_out")] +
+                         [(trim, n) for n in ("lengths_in", "lengths_out", "next_positions", "weights_in", "weights_out", "positions_in", "positions_out")])
+def test_lists_off_a_word_boundary(L, call, name):
+    assert call(L, **{name: 0x900002}) == INVALID and b"4-byte" in L.qllm_last_error()
