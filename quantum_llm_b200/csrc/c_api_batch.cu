@@ -30,8 +30,22 @@ size_t row_bytes(uint32_t type) { return type == QLLM_ROW_F32 ? 4U : 2U; }
 // Whether `rows` rows `stride` elements apart can be addressed at all.
 bool extent_ok(size_t rows, size_t stride) { return stride <= (static_cast<size_t>(1) << 56U) / rows; }
 
-// Elements from the first to the last of `rows` rows of `width`.
-size_t extent(size_t rows, size_t stride, size_t width) { return (rows - 1U) * stride + width; }
+// `count` rows of `width` elements of `size` bytes, `stride` elements apart; the strides have passed extent_ok.
+struct Rows {
+  const void* p;
+  size_t count, stride, width, size;
+  size_t bytes() const { return ((count - 1U) * stride + width) * size; }
+};
+// Whether two sets of rows share memory.  Rows of one stride may be columns of one buffer; of different strides the space
+// between the rows counts as theirs.
+bool overlap(const Rows& a, const Rows& b) {
+  if (!overlap(a.p, a.bytes(), b.p, b.bytes())) return false;
+  const size_t period = a.stride * a.size;
+  if (period != b.stride * b.size) return true;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  const size_t after = y >= x ? (y - x) % period : (period - (x - y) % period) % period;  // from a row of a to the next of b
+  return after < a.width * a.size || after + b.width * b.size > period;
+}
 
 // Geometry of the cache; 0 or the refusal.
 int check_cache(const qllm_kv_batch* c, const char* who) {
@@ -119,14 +133,11 @@ int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, con
                          !extent_ok(static_cast<size_t>(cache->sequences) * cache->kv_heads, slot_stride)))
     return fail(QLLM_INVALID_ARGUMENT, "QK norm / RoPE / KV store: slot_positions needs row_slot and a stride that holds every slot");
   // in place is every row's own head over itself; any other sharing would be overwritten before it is read
-  const size_t in = extent(rows, qkv_stride, q_width + 2U * kv_width) * e;
-  const size_t q_out = extent(rows, query_stride, q_width) * e, k_out = key ? extent(rows, key_stride, kv_width) * e : 0U;
-  const uint8_t* base = static_cast<const uint8_t*>(qkv);
+  const Rows in{qkv, rows, qkv_stride, q_width + 2U * kv_width, e}, q_out{query, rows, query_stride, q_width, e},
+      k_out{key, rows, key_stride, kv_width, e};
   const bool query_in_place = query == qkv && query_stride == qkv_stride;
-  const bool key_in_place = key == base + q_width * e && key_stride == qkv_stride;
-  const bool both_in_place = query_in_place && key_in_place;
-  if ((!query_in_place && overlap(query, q_out, qkv, in)) || (key && !key_in_place && overlap(key, k_out, qkv, in)) ||
-      (key && !both_in_place && overlap(key, k_out, query, q_out)))
+  const bool key_in_place = key == static_cast<const uint8_t*>(qkv) + q_width * e && key_stride == qkv_stride;
+  if ((!query_in_place && overlap(q_out, in)) || (key && !key_in_place && overlap(k_out, in)) || (key && overlap(k_out, q_out)))
     return fail(QLLM_INVALID_ARGUMENT, "QK norm / RoPE / KV store: rows overlap and are not in place");
   if ((rc = check_device(qkv, who))) return rc;
   NormRopeStoreArgs a{*cache, row_type, qkv, qkv_stride, rows, q_heads, rotary_dim, q_norm, k_norm, eps, inv_freq, positions,
@@ -154,14 +165,16 @@ int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const
   if (!rows_ok(query, cache->sequences, query_stride, row_type, width) || !rows_ok(out, cache->sequences, out_stride, row_type, width))
     return fail(QLLM_INVALID_ARGUMENT,
                 "decode attention needs rows on 16-byte boundaries, strides that hold a row and are multiples of 16 bytes");
-  if (overlap(query, extent(cache->sequences, query_stride, width) * e, out, extent(cache->sequences, out_stride, width) * e))
+  if (overlap(Rows{query, cache->sequences, query_stride, width, e}, Rows{out, cache->sequences, out_stride, width, e}))
     return fail(QLLM_INVALID_ARGUMENT, "decode attention: query and out overlap");
   if (weights_in && !weights_out) return fail(QLLM_INVALID_ARGUMENT, "decode attention: weights_in without weights_out");
   if (weights_out) {
     if (weights_stride < kv_capacity(*cache) || !extent_ok(static_cast<size_t>(cache->sequences) * cache->kv_heads, weights_stride))
       return fail(QLLM_INVALID_ARGUMENT, "decode attention: the weights' stride does not hold every slot");
-    const size_t bytes = extent(static_cast<size_t>(cache->sequences) * cache->kv_heads, weights_stride, kv_capacity(*cache)) * sizeof(float);
-    if (weights_in && weights_in != weights_out && overlap(weights_in, bytes, weights_out, bytes))
+    const auto array = [&](const void* p) {
+      return Rows{p, static_cast<size_t>(cache->sequences) * cache->kv_heads, weights_stride, kv_capacity(*cache), sizeof(float)};
+    };
+    if (weights_in && weights_in != weights_out && overlap(array(weights_in), array(weights_out)))
       return fail(QLLM_INVALID_ARGUMENT, "decode attention: weights overlap and are not in place");
   }
   if (!aligned(workspace, 16U) || workspace_bytes < decode_attention_workspace_bytes(*cache, q_heads, weights_out != nullptr))
@@ -192,11 +205,11 @@ int qllm_k_kv_evict(const qllm_kv_batch* cache, const uint32_t* lengths_in, uint
     return fail(QLLM_INVALID_ARGUMENT, "KV eviction needs a budget that holds the recent tokens and the sinks");
   if (stride < kv_capacity(*cache) || !extent_ok(static_cast<size_t>(cache->sequences) * cache->kv_heads, stride))
     return fail(QLLM_INVALID_ARGUMENT, "KV eviction: the stride does not hold every slot");
-  const size_t bytes = extent(static_cast<size_t>(cache->sequences) * cache->kv_heads, stride, kv_capacity(*cache)) * 4U;
-  if ((weights_in != weights_out && overlap(weights_in, bytes, weights_out, bytes)) ||
-      (positions_in != positions_out && overlap(positions_in, bytes, positions_out, bytes)) ||
-      overlap(weights_out, bytes, positions_in, bytes) || overlap(weights_out, bytes, positions_out, bytes) ||
-      overlap(weights_in, bytes, positions_out, bytes))
+  const auto array = [&](const void* p) { return Rows{p, static_cast<size_t>(cache->sequences) * cache->kv_heads, stride, kv_capacity(*cache), 4U}; };
+  if ((weights_in != weights_out && overlap(array(weights_in), array(weights_out))) ||
+      (positions_in != positions_out && overlap(array(positions_in), array(positions_out))) ||
+      overlap(array(weights_out), array(positions_in)) || overlap(array(weights_out), array(positions_out)) ||
+      overlap(array(weights_in), array(positions_out)))
     return fail(QLLM_INVALID_ARGUMENT, "KV eviction: arrays overlap and are not in place");
   const size_t list = cache->sequences * sizeof(uint32_t);
   if ((lengths_in != lengths_out && overlap(lengths_in, list, lengths_out, list)) || overlap(next_positions, list, lengths_out, list))

@@ -148,3 +148,35 @@ def test_no_workspace_for_query_heads_that_the_attention_refuses(L, q_heads, ove
                          [(trim, n) for n in ("lengths_in", "lengths_out", "next_positions", "weights_in", "weights_out", "positions_in", "positions_out")])
 def test_lists_off_a_word_boundary(L, call, name):
     assert call(L, **{name: 0x900002}) == INVALID and b"4-byte" in L.qllm_last_error()
+
+
+SIDE_BY_SIDE = [
+    # query and key rows as columns of one buffer; both behind the row in a wider buffer; key before query
+    (store, dict(query=0x200000, query_stride=6 * 128, key=0x200000 + 8 * 128, key_stride=6 * 128)),
+    (store, dict(qkv_stride=14 * 128, query=0x100000 + 16 * 128, query_stride=14 * 128, key=0x100000 + 24 * 128, key_stride=14 * 128)),
+    (store, dict(query=0x200000 + 4 * 128, query_stride=6 * 128, key=0x200000, key_stride=6 * 128)),
+    (attend, dict(query=0x100000, query_stride=8 * 128, out=0x100000 + 8 * 128, out_stride=8 * 128)),
+    (attend, dict(weights_in=0x400000, weights_out=0x400000 + 256 * 4, weights_stride=512)),
+    (trim, dict(weights_in=0x400000, weights_out=0x400000, positions_in=0x400000 + 256 * 4, positions_out=0x400000 + 256 * 4, stride=512))]
+ONE_OVER_ANOTHER = [
+    (store, dict(query=0x200000, query_stride=6 * 128, key=0x200000 + 8 * 128 - 16, key_stride=6 * 128)),
+    (store, dict(query=0x200000, query_stride=6 * 128, key=0x200000 + 8 * 128 + 16, key_stride=6 * 128)),       # its end over the next row
+    (store, dict(query=0x200000, query_stride=6 * 128, key=0x200000 + 8 * 128, key_stride=12 * 128)),
+    (store, dict(qkv_stride=14 * 128, query=0x100000 + 16 * 128 - 16, query_stride=14 * 128)),
+    (attend, dict(query=0x100000, query_stride=8 * 128, out=0x100000 + 8 * 128 + 16, out_stride=8 * 128)),
+    (attend, dict(query=0x100000, query_stride=8 * 128, out=0x100000 - 8 * 128 - 16, out_stride=8 * 128)),
+    (attend, dict(weights_in=0x400000, weights_out=0x400000 + 255 * 4, weights_stride=512)),
+    (trim, dict(weights_in=0x400000, weights_out=0x400000, positions_in=0x400000 + 257 * 4, positions_out=0x400000 + 257 * 4, stride=512))]
+
+
+@pytest.mark.parametrize("call,over", SIDE_BY_SIDE)
+def test_columns_of_one_buffer_do_not_overlap(L, call, over):
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses that pass the checks; test_gpu_batch_paths.py has the calls on a GPU")
+    assert call(L, **over) != INVALID
+
+
+@pytest.mark.parametrize("call,over", ONE_OVER_ANOTHER)
+def test_columns_that_overlap_are_refused(L, call, over):
+    assert call(L, **over) == INVALID and b"overlap" in L.qllm_last_error()
