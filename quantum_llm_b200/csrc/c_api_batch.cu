@@ -1,6 +1,7 @@
 // extern "C" forms of the operators for batches of sequences (include/qllm_b200.h): every argument
 // that the host can see is checked here, before any CUDA call.
 #include <cmath>
+#include <initializer_list>
 #include <string>
 
 #include "kernels.h"
@@ -87,18 +88,26 @@ bool rows_ok(const void* p, size_t rows, size_t stride, uint32_t type, size_t wi
 }
 
 // The call's memory has to be the current device's: a host pointer, or another device's memory, would fault in the kernel.
-// One pointer stands for all of a call's (some 0.2 us).
-int check_device(const void* p, const char* what) {
-  cudaPointerAttributes attributes{};
+// The rows or page tables stand for all of a call's memory, and one list for its lists, which are what a host has at hand (0.15 us a
+// pointer; all pointers of a call would be 0.9 us of some 5).  Lists may lie in pinned host memory, which the device reads as it is.
+int check_device(const char* what, std::initializer_list<const void*> memory, const void* list) {
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess) e = cudaPointerGetAttributes(&attributes, p);
+  bool there = true;
+  const auto check = [&](const void* p, bool pinned) {
+    if (e != cudaSuccess || !there || !p) return;
+    cudaPointerAttributes attributes{};
+    e = cudaPointerGetAttributes(&attributes, p);
+    there = (attributes.type == cudaMemoryTypeDevice && attributes.device == device) || attributes.type == cudaMemoryTypeManaged ||
+            (pinned && attributes.type == cudaMemoryTypeHost);
+  };
+  for (const void* p : memory) check(p, false);
+  check(list, true);
   if (e != cudaSuccess) {
     cudaGetLastError();  // reported here, not by the next call
     return check_cuda(e, what);
   }
-  if ((attributes.type == cudaMemoryTypeDevice && attributes.device == device) || attributes.type == cudaMemoryTypeManaged) return 0;
-  return fail(QLLM_INVALID_ARGUMENT, std::string(what) + ": the call's memory is not the current device's");
+  return there ? 0 : fail(QLLM_INVALID_ARGUMENT, std::string(what) + ": the call's memory is not the current device's");
 }
 
 }  // namespace
@@ -139,7 +148,7 @@ int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, con
   const bool key_in_place = key == static_cast<const uint8_t*>(qkv) + q_width * e && key_stride == qkv_stride;
   if ((!query_in_place && overlap(q_out, in)) || (key && !key_in_place && overlap(k_out, in)) || (key && overlap(k_out, q_out)))
     return fail(QLLM_INVALID_ARGUMENT, "QK norm / RoPE / KV store: rows overlap and are not in place");
-  if ((rc = check_device(qkv, who))) return rc;
+  if ((rc = check_device(who, {qkv, row_slot ? cache->page_tables : nullptr}, positions))) return rc;
   NormRopeStoreArgs a{*cache, row_type, qkv, qkv_stride, rows, q_heads, rotary_dim, q_norm, k_norm, eps, inv_freq, positions,
                       row_sequence, row_slot, query, query_stride, key, key_stride, slot_positions, slot_stride};
   return launch_norm_rope_store(a, static_cast<cudaStream_t>(stream));
@@ -179,7 +188,7 @@ int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const
   }
   if (!aligned(workspace, 16U) || workspace_bytes < decode_attention_workspace_bytes(*cache, q_heads, weights_out != nullptr))
     return fail(QLLM_INVALID_ARGUMENT, "decode attention workspace is too small or not on a 16-byte boundary");
-  if ((rc = check_device(cache->page_tables, who))) return rc;
+  if ((rc = check_device(who, {cache->page_tables}, lengths))) return rc;
   DecodeAttentionArgs a{*cache, row_type, query, query_stride, lengths, q_heads, scale, weights_in, weights_out, weights_stride,
                         out, out_stride, workspace};
   return launch_decode_attention(a, static_cast<cudaStream_t>(stream));
@@ -216,7 +225,7 @@ int qllm_k_kv_evict(const qllm_kv_batch* cache, const uint32_t* lengths_in, uint
     return fail(QLLM_INVALID_ARGUMENT, "KV eviction: arrays overlap and are not in place");
   if (!aligned(workspace, 16U) || workspace_bytes < kv_evict_workspace_bytes(*cache, budget))
     return fail(QLLM_INVALID_ARGUMENT, "KV eviction workspace is too small or not on a 16-byte boundary");
-  if ((rc = check_device(cache->page_tables, who))) return rc;
+  if ((rc = check_device(who, {cache->page_tables}, lengths_in))) return rc;
   KvEvictArgs a{*cache, lengths_in, lengths_out, next_positions, budget, recent, sinks, weights_in, weights_out, positions_in,
                 positions_out, stride, workspace};
   return launch_kv_evict(a, static_cast<cudaStream_t>(stream));

@@ -59,3 +59,41 @@ def test_weights_and_positions_as_columns_of_one_buffer():
             assert torch.equal(weights[s, h, :m], w[s, h][at]) and torch.equal(positions[s, h, :m], p[s, h][at])
             assert torch.equal(after[s, :m, h], before[s, at, h]) and bool((weights[s, h, m:full] == 0).all())
             assert torch.equal(weights[s, h, full:], w[s, h, full:]) and torch.equal(positions[s, h, m:], p[s, h, m:])
+
+
+# ------------------------------------------------------------------------- memory of the host
+
+def test_lists_and_page_tables_of_the_host_are_refused():
+    """Pageable host memory: refused before any launch.  Pinned lists are read as they are."""
+    q, kv, hd = 4, 2, 64
+    cache = PagedCache(2, 2, 16, F16, kv, hd, seed=3)
+    host, table = cache.descriptor(), cache.tables.cpu()
+    host.page_tables = table.data_ptr()
+    L, n, kept, following = bc.ql.load(), u32([5, 20]), u32([0, 0]), u32([5, 20])
+    far = n.cpu()
+    pinned = far.pin_memory()
+    x = rand((2, (q + 2 * kv) * hd), 1)
+    query, out, ws = rand((2, q * hd), 2), torch.zeros(2, q * hd, device="cuda"), bc.attention_workspace(cache, q, False)
+    w, p = torch.zeros(2, kv, 32, device="cuda"), torch.zeros(2, kv, 32, dtype=torch.int32, device="cuda")
+    norm = torch.ones(hd, device="cuda")
+
+    def store(descriptor, positions):
+        return L.qllm_k_qk_norm_rope_store(descriptor, 0, x.data_ptr(), x.stride(0), 2, q, 0, norm.data_ptr(), norm.data_ptr(), 1e-6, None,
+                                           positions.data_ptr(), None, n.data_ptr(), query.data_ptr(), q * hd, None, 0, None, 0, bc.stream())
+
+    def attend(lengths):
+        return L.qllm_k_decode_attention(cache.descriptor(), 0, query.data_ptr(), q * hd, lengths.data_ptr(), q, 0.1, None, None, 0,
+                                         out.data_ptr(), q * hd, ws.data_ptr(), ws.numel(), bc.stream())
+
+    def trim(lengths):
+        return L.qllm_k_kv_evict(cache.descriptor(), lengths.data_ptr(), kept.data_ptr(), following.data_ptr(), 4, 0, 0, w.data_ptr(), w.data_ptr(),
+                                 p.data_ptr(), p.data_ptr(), 32, ws.data_ptr(), ws.numel(), bc.stream())
+
+    before = [t.clone() for t in (cache.pool, query, out, w, p, kept)]
+    for refused in (store(host, n), store(cache.descriptor(), far), attend(far), trim(far)):
+        assert refused == -4 and b"current device" in L.qllm_last_error()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, (cache.pool, query, out, w, p, kept)))
+    assert attend(pinned) == 0
+    torch.cuda.synchronize()
+    check_attention(cache, query, [5, 20], q, 0.1, out, None, None, F32)
