@@ -97,3 +97,151 @@ def test_lists_and_page_tables_of_the_host_are_refused():
     assert attend(pinned) == 0
     torch.cuda.synchronize()
     check_attention(cache, query, [5, 20], q, 0.1, out, None, None, F32)
+
+
+# ------------------------------------------------------------------------- the pages of the single-stream calls
+
+@pytest.mark.parametrize("enc", [F16, Q4H, Q8])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attention_reads_records_of_the_single_stream_store(enc, hd):
+    """qllm_k_rope_kv_store writes two sequences' rows, one decode attention reads them."""
+    q, kv, page, lengths = 4, 2, 64, [130, 61]
+    cache = PagedCache(2, 3, page, enc, kv, hd, layers=2, layer=1, seed=3, fill=False)
+    L, inv = bc.ql.load(), inv_freq(hd)
+    top = {F16: 2.0 ** 11, Q4H: 7.0, Q8: 127.0}[enc]
+    for s, n in enumerate(lengths):
+        rows = rand((n, (q + 2 * kv) * hd), 10 + s)
+        kept = rows.view(n, q + 2 * kv, hd)[:, q:].double()
+        at = u32([0])
+        bc.ql.check(L.qllm_k_rope_kv_store(rows.data_ptr(), n, q, kv, hd, 0, inv.data_ptr(), at.data_ptr(), 0, 0, cache.tables[s].data_ptr(),
+                                           cache.layer * cache.bytes, page, enc, 0, bc.stream()))
+        torch.cuda.synchronize()
+        k, v, _ = cache.values(s, n)
+        step = kept.abs().amax(-1, keepdim=True) / top      # a record is within a step of its row
+        assert bool(((torch.cat((k, v), 1) - kept).abs() <= step).all())
+    query = rand((2, q * hd), 5, 2.0)
+    out, weights = torch.zeros(2, q * hd, device="cuda"), torch.full((2, kv, cache.capacity), -3.0, device="cuda")
+    bc.decode_attention(cache, query, u32(lengths), q, hd ** -0.5, out, None, weights)
+    torch.cuda.synchronize()
+    check_attention(cache, query, lengths, q, hd ** -0.5, out, None, weights, F32)
+
+
+@pytest.mark.parametrize("enc", [F16, Q4H, Q8])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_single_stream_attention_reads_records_of_the_batched_store(enc, hd):
+    """qllm_k_qk_norm_rope_store writes two sequences' rows, qllm_k_attention reads each.  Its weights may be INT8 relative to the
+    largest: off by 1 / 127 / sqrt(12) of it a key (each by itself), which meets a value of V's root mean square; four times the
+    norm of that is allowed, and a BF16 step of the outputs."""
+    q, kv, page, n = 4, 2, 64, 97
+    cache = PagedCache(2, 2, page, enc, kv, hd, layers=2, layer=1, seed=3, fill=False)
+    x = rand((2 * n, (q + 2 * kv) * hd), 3)
+    w, inv = 1 + 0.1 * rand(hd, 4), inv_freq(hd)
+    rows = torch.zeros(2 * n, q * hd, device="cuda")
+    order = list(range(n))
+    bc.norm_rope_store(cache, x, q, hd, w, w, inv, u32(order + order), u32([0] * n + [1] * n), u32(order + order), rows)
+    L, split, splits = bc.ql.load(), 64, 3
+    space = torch.empty(L.qllm_k_attention_workspace_bytes(1, q, hd, splits), dtype=torch.uint8, device="cuda")
+    out, at = torch.zeros(1, q * hd, device="cuda"), u32([n - 1])
+    for s in range(2):
+        query = rows[s * n + n - 1:s * n + n].contiguous()
+        bc.ql.check(L.qllm_k_attention(enc, cache.tables[s].data_ptr(), cache.layer * cache.bytes, page, query.data_ptr(), q * hd, 1, at.data_ptr(), 0,
+                                       q, kv, hd, split, splits, 0, space.data_ptr(), out.data_ptr(), 0, bc.stream()))
+        torch.cuda.synchronize()
+        want, p, _, _, _ = bc.exact_attention(cache, s, n, query[0], q, hd ** -0.5)
+        values = cache.values(s, n)[1]
+        allowed = 4 * p.amax(-1) / 127 / 12 ** 0.5 * float(values.square().mean().sqrt()) * (n * hd) ** 0.5 + 2.0 ** -7 * want.norm(dim=-1)
+        assert bool(((out.view(q, hd).double() - want).norm(dim=-1) <= allowed).all())
+        # records read a slot further on would show
+        wrong = torch.einsum("hgt,thd->hgd", p.view(kv, q // kv, n), values.roll(1, 0)).reshape(q, hd)
+        assert bool(((wrong - want).norm(dim=-1) > allowed).all())
+
+
+# ------------------------------------------------------------------------- batch sizes that choose another path
+
+def blocks_of(cache, lengths, q_heads):
+    """(items, items that more than one block of the attention's first launch works on), from its rule: equal shares of a line of 64-token
+    units, an item's own cost before its tokens."""
+    heads = 1 if cache.enc != Q8 else 4 if cache.kv % 4 == 0 else 2 if cache.kv % 2 == 0 else 1
+    unit = 64 * heads * bc.layer_bytes(cache.enc, 1, 1, cache.hd)
+    cost, tiles = -(-96 * 1024 // unit), -(-(q_heads // cache.kv) // 8)
+    sizes = [-(-n // 64) + cost for n in lengths if n for _ in range(cache.kv // heads * tiles)]
+    total = sum(sizes)
+    per_sm = {64: 4, 128: 3}.get(cache.hd, 2)
+    blocks = min(768, torch.cuda.get_device_properties(0).multi_processor_count * per_sm, total)
+    at, split = 0, 0
+    for n in sizes:
+        first, last = at + cost, at + n - 1
+        split += ((first + 1) * blocks - 1) // total != ((last + 1) * blocks - 1) // total
+        at += n
+    return len(sizes), split
+
+
+@pytest.mark.parametrize("q,kv,hd,enc,dtype", [(32, 4, 64, F16, BF16), (32, 4, 128, F16, F32), (40, 8, 64, Q8, HF16), (24, 2, 192, Q4H, BF16), (24, 4, 256, Q8, F32)])
+@pytest.mark.parametrize("weights", [False, True])
+def test_attention_of_many_query_heads(q, kv, hd, enc, dtype, weights):
+    """More than eight query heads to a multiprocessor, where one warp joins a head's parts instead of four, and items that blocks share."""
+    sequences, page, top = 1300 // q + 14, 64, 3000
+    lengths = [top, 0, 1] + [int(top * ((37 * s) % 101) / 101) + 200 for s in range(sequences - 4)] + [top - 1]
+    lengths = [min(n, top) for n in lengths]
+    cache = PagedCache(sequences, -(-top // page), page, enc, kv, hd, seed=3)
+    assert sequences * q > 8 * torch.cuda.get_device_properties(0).multi_processor_count
+    items, split = blocks_of(cache, lengths, q)
+    assert split > items // 4
+    query = rand((sequences, q * hd), 9, 2.0).to(dtype)
+    out = torch.full((sequences, q * hd), 7.0, dtype=dtype, device="cuda")
+    w_out = torch.full((sequences, kv, cache.capacity), -3.0, device="cuda") if weights else None
+    bc.decode_attention(cache, query, u32(lengths), q, hd ** -0.5, out, None, w_out)
+    torch.cuda.synchronize()
+    check_attention(cache, query, lengths, q, hd ** -0.5, out, None, w_out, dtype)
+    assert bool((out[1] == 0).all())
+
+
+@pytest.mark.parametrize("q,kv,enc,dtype", [(8, 8, F16, BF16), (48, 4, Q8, F32)])
+def test_weights_of_many_rows(q, kv, enc, dtype):
+    """More chunks of 512 tokens in a row than blocks that add up its weights (some 16 to a multiprocessor over all rows); the second
+    case has more than eight query heads to a kv head, whose weights are added to the first ones'."""
+    sequences, hd, page, top = 1280 // kv, 64, 64, 1700
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert -(-16 * sms // (sequences * kv)) < -(-top // 512)
+    lengths = [(top * (s % 41)) // 40 for s in range(sequences)]
+    cache = PagedCache(sequences, -(-top // page), page, enc, kv, hd, seed=3)
+    query = rand((sequences, q * hd), 9, 2.0).to(dtype)
+    out = torch.zeros((sequences, q * hd), dtype=dtype, device="cuda")
+    w_in, w_out = torch.rand(sequences, kv, cache.capacity, device="cuda"), torch.full((sequences, kv, cache.capacity), -3.0, device="cuda")
+    bc.decode_attention(cache, query, u32(lengths), q, hd ** -0.5, out, w_in, w_out)
+    torch.cuda.synchronize()
+    check_attention(cache, query, lengths, q, hd ** -0.5, out, w_in, w_out, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, HF16])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("rot", [128, 32])
+def test_norm_rope_store_of_many_passes(dtype, in_place, rot):
+    """Rows enough for ten passes to a warp (2048 warps for 1500 rows of 56 heads, four to a pass): the values copied ahead wrap round."""
+    q, kv, hd, rows, page = 40, 8, 128, 1500, 64
+    assert (q + 2 * kv) // 4 * rows // 2048 >= 10
+    cache = PagedCache(1, -(-rows // page), page, F16, kv, hd, seed=3)
+    x = rand((rows, (q + 2 * kv) * hd), 8).to(dtype)
+    given = x.clone()
+    q_norm, k_norm, inv = 1 + 0.2 * rand(hd, 4), 1 + 0.2 * rand(hd, 5), inv_freq(rot)
+    slot = list(range(rows))
+    slot[7] = slot[900] = slot[rows - 1] = 0xFFFFFFFF
+    if in_place:
+        query, key = x, x[:, q * hd:(q + kv) * hd]
+    else:
+        query, key = torch.full((rows, q * hd), 7.0, dtype=dtype, device="cuda"), torch.full((rows, kv * hd), 7.0, dtype=dtype, device="cuda")
+    before = cache.records()
+    bc.norm_rope_store(cache, x, q, rot, q_norm, k_norm, inv, u32(range(rows)), u32([0] * rows), u32(slot), query, key)
+    torch.cuda.synchronize()
+    wq, wk, size = bc.exact_norm_rope(given, q, kv, hd, rot, q_norm, k_norm, inv, range(rows))
+    live = torch.tensor([s != 0xFFFFFFFF for s in slot], device="cuda")
+    close_norm(query[:, :q * hd].reshape(rows, q, hd)[live], wq[live], size[live][:, :q], dtype)
+    close_norm(key.reshape(rows, kv, hd)[live], wk[live], size[live][:, q:], dtype)
+    k, v, _ = cache.values(0, rows)
+    close_norm(k[live].half(), wk[live], size[live][:, q:], HF16)
+    assert torch.equal(v[live], given.view(rows, q + 2 * kv, hd)[live][:, q + kv:].half().double())
+    assert torch.equal(cache.records()[0, :rows][~live], before[0, :rows][~live])
+    if in_place:
+        assert torch.equal(x[~live], given[~live]) and torch.equal(x[:, (q + kv) * hd:], given[:, (q + kv) * hd:])
+    else:
+        assert torch.equal(x, given) and bool((query[~live] == 7).all()) and bool((key[~live] == 7).all())
