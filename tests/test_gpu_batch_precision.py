@@ -136,6 +136,41 @@ def test_attention_behind_a_key_that_adds_nothing(dtype, gap, n):
     check(out[0].view(q, hd), want, dtype, 8 * E * gap)
 
 
+@pytest.mark.parametrize("enc", [Q4H, Q8])
+@pytest.mark.parametrize("gap", [10.0, 16.0, 20.0])
+def test_attention_behind_a_quantised_key_that_adds_nothing(enc, gap):
+    """The same over quantised caches, whose V scale counts into the reference: the sink's is the smallest there is, 2^-24.  At 20 nats
+    the others' weight times scale (at least 2^-6) is above 2^-11 of the sink's, to which two F16 terms hold 22 bits."""
+    q, kv, hd, page, n = 8, 2, 128, 64, 2048
+    cache = PagedCache(1, n // page, page, enc, kv, hd, seed=5)
+    half, records, at = cache.bytes // 2, page * kv, int(cache.index[0, 0])
+    pool = cache.pool.view(-1, 2, half)
+    query = rand((1, q * hd), 4)
+    query[0].view(q, hd)[:, 0] = 8.0
+    codes = 127 if enc == Q8 else 7
+    for h in range(kv):
+        # dimension 0 carries the gap alone: zero for every other key, the largest code for the first one
+        if enc == Q8:
+            token_major = pool.view(-1, 2, page, kv, hd + 2)
+            token_major[:, 0, :, h, 0] = 0
+            token_major[at, :, 0, h, :hd] = 0
+            token_major[at, 0, 0, h, 0] = codes
+            scales = cache.pool.view(HF16).view(-1, 2, page, kv, hd // 2 + 1)[at, :, 0, h, hd // 2]
+        else:
+            nibbles = pool[:, :, :records * hd // 2].view(-1, 2, kv, page, hd // 2)
+            nibbles[:, 0, h, :, 0] &= 0xF0
+            nibbles[at, :, h, 0] = 0
+            nibbles[at, 0, h, 0, 0] = codes
+            scales = pool[:, :, records * hd // 2:].view(HF16).view(-1, 2, kv, page)[at, :, h, 0]
+        scales[0] = gap * hd ** 0.5 / 8.0 / codes
+        scales[1] = 2.0 ** -24
+    out = torch.zeros((1, q * hd), device="cuda")
+    bc.decode_attention(cache, query, u32([n]), q, hd ** -0.5, out)
+    torch.cuda.synchronize()
+    want = bc.exact_attention(cache, 0, n, query[0], q, hd ** -0.5)[0]
+    check(out[0].view(q, hd), want, F32, 8 * E * gap)
+
+
 @pytest.mark.parametrize("q,kv,hd,enc,dtype", [(8, 4, 64, Q8, HF16), (8, 1, 64, F16, HF16), (8, 1, 128, Q4H, HF16), (8, 4, 128, Q8, F32),
                                                (8, 1, 64, F16, F32), (8, 1, 64, Q4H, F32)])
 def test_attention_of_long_items_that_no_block_shares(q, kv, hd, enc, dtype):
