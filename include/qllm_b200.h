@@ -481,7 +481,8 @@ typedef struct qllm_kv_batch {
  * (gated_gqa_qkv_rope_paged_batch_kernel with its per-head norm, transformer_kernels.cu:3551-3643,
  * for rows of many sequences).  Row r of qkv [rows, (q_heads + 2 kv_heads) * head_dim] (row_type values,
  * qkv_stride elements apart):
- *   n = x * w / sqrt(mean(x^2) + eps) per query head (w = q_norm) and key head (w = k_norm), [head_dim] FP32;
+ *   n = x * w / sqrt(mean(x^2) + eps) per query head (w = q_norm) and key head (w = k_norm), [head_dim] FP32; q_norm and
+ *   k_norm both null: n = x, for models without a per-head norm;
  *   the first rotary_dim values (a multiple of 16, may be 0) are rotated in pairs (i, i + rotary_dim / 2)
  *   by positions[r] * inv_freq[i], the angle reduced in FP64;
  *   query [rows, q_heads * head_dim], and key [rows, kv_heads * head_dim] unless it is null, get the

@@ -124,7 +124,7 @@ int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, con
   int rc = check_cache(cache, who);
   if (rc) return rc;
   if (row_slot && (rc = check_pages(cache, who))) return rc;
-  if (!rows || !q_heads || q_heads > 65536U || row_type > QLLM_ROW_F16 || !q_norm || !k_norm || !positions ||
+  if (!rows || !q_heads || q_heads > 65536U || row_type > QLLM_ROW_F16 || !q_norm != !k_norm || !positions ||
       !(eps >= 0.0F) || std::isinf(eps))
     return fail(QLLM_INVALID_ARGUMENT, "invalid QK norm / RoPE / KV store batch");
   if ((rc = check_words(who, q_norm, k_norm, inv_freq, positions, row_sequence, row_slot, slot_positions))) return rc;

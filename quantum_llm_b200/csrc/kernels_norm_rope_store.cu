@@ -1,7 +1,7 @@
 // Per-head RMS norm of queries and keys, rotation by position and the K/V records, for rows of many
 // sequences in one launch (qllm_k_qk_norm_rope_store).
 //
-//   n_d = x_d * w_d / sqrt(mean_d x_d^2 + eps)                      over the head's D values
+//   n_d = x_d * w_d / sqrt(mean_d x_d^2 + eps)                      over the head's D values (without weights: n = x)
 //   y_i = n_i cos a_i - n_{i+R/2} sin a_i,  y_{i+R/2} = n_{i+R/2} cos a_i + n_i sin a_i,  i < R/2
 //   a_i = position * inv_freq[i];  y_d = n_d for d >= R
 //
@@ -94,7 +94,7 @@ norm_rope_store_kernel(const __grid_constant__ NormRopeStoreArgs a, uint32_t tas
   __shared__ alignas(16) float norm[2][HD];
   extern __shared__ uint4 ring_memory[];                       // a lane's values of the passes to come; nobody else reads them
   uint4 (&ring)[kStages][2U * kWords][kThreads] = *reinterpret_cast<uint4 (*)[kStages][2U * kWords][kThreads]>(ring_memory);
-  for (uint32_t i = threadIdx.x; i < 2U * HD; i += kThreads) norm[i / HD][i % HD] = (i < HD ? a.q_norm : a.k_norm)[i % HD];
+  for (uint32_t i = threadIdx.x; i < 2U * HD; i += kThreads) norm[i / HD][i % HD] = a.q_norm ? (i < HD ? a.q_norm : a.k_norm)[i % HD] : 1.0F;
   __syncthreads();
   const uint64_t task = static_cast<uint64_t>(blockIdx.x) * (kThreads / 32U) + (threadIdx.x >> 5U);
   const uint32_t row = static_cast<uint32_t>(task / tasks_per_row);
@@ -176,7 +176,7 @@ norm_rope_store_kernel(const __grid_constant__ NormRopeStoreArgs a, uint32_t tas
       sum = head_sum<kLanes>(sum);
       if (live && !is_value) {
         const float* w = norm[head < a.q_heads ? 0 : 1];
-        const float r = rsqrtf(fmaf(sum, 1.0F / HD, a.eps));
+        const float r = a.q_norm ? rsqrtf(fmaf(sum, 1.0F / HD, a.eps)) : 1.0F;
         float w0[8], w1[8];
         load8(w + 8U * c0, w0);
         load8(w + 8U * c1, w1);

@@ -97,7 +97,7 @@ struct NormRopeStoreArgs {
   const void* qkv;           // [rows, (q + 2 kv) * head_dim], rows qkv_stride elements apart
   size_t qkv_stride;
   uint32_t rows, q_heads, rotary_dim;
-  const float* q_norm;       // [head_dim]
+  const float* q_norm;       // [head_dim]; both null: no norm
   const float* k_norm;
   float eps;
   const float* inv_freq;     // [rotary_dim / 2]

@@ -180,3 +180,11 @@ def test_columns_of_one_buffer_do_not_overlap(L, call, over):
 @pytest.mark.parametrize("call,over", ONE_OVER_ANOTHER)
 def test_columns_that_overlap_are_refused(L, call, over):
     assert call(L, **over) == INVALID and b"overlap" in L.qllm_last_error()
+
+
+def test_rows_without_norm_weights_are_taken(L):
+    """Both null: no norm.  One alone is refused (test_norm_rope_store)."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses that pass the checks; test_gpu_batch_paths.py has the call on a GPU")
+    assert store(L, q_norm=None, k_norm=None) != INVALID

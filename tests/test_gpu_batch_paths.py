@@ -99,6 +99,39 @@ def test_lists_and_page_tables_of_the_host_are_refused():
     check_attention(cache, query, [5, 20], q, 0.1, out, None, None, F32)
 
 
+# ------------------------------------------------------------------------- models without a per-head norm
+
+@pytest.mark.parametrize("q,kv,hd,rot,dtype,enc,page", [(40, 8, 128, 128, BF16, Q4H, 256), (32, 4, 128, 128, HF16, F16, 64), (12, 2, 256, 64, F32, Q8, 16),
+                                                        (5, 1, 64, 0, BF16, F16, 48), (3, 3, 192, 96, F32, Q4H, 32)])
+def test_rope_store_without_norm_weights(q, kv, hd, rot, dtype, enc, page):
+    """q_norm and k_norm null: rotation and records of the rows as they are, whatever eps is; without a rotation the outputs are the inputs."""
+    rows, sequences = 37, 3
+    cache = PagedCache(sequences, 4, page, enc, kv, hd, layers=2, layer=1, seed=rows)
+    x = rand((rows, (q + 2 * kv) * hd), 5, 1.5).to(dtype)
+    x[3] = 0
+    inv, position = inv_freq(rot), [[0, 1, 4095, 1_000_003, 4_000_000_000][r % 5] + r for r in range(rows)]
+    sequence, slot = [r % sequences for r in range(rows)], [r // sequences for r in range(rows)]
+    query, key = torch.zeros(rows, q * hd, dtype=dtype, device="cuda"), torch.zeros(rows, kv * hd, dtype=dtype, device="cuda")
+    for eps in (0.0, 1e-6):
+        bc.norm_rope_store(cache, x, q, rot, None, None, inv, u32(position), u32(sequence), u32(slot), query, key, eps=eps)
+        torch.cuda.synchronize()
+        heads = x.double().view(rows, q + 2 * kv, hd)[:, :q + kv]
+        want, size, half = heads.clone(), heads.abs(), rot // 2
+        if half:
+            angle = torch.tensor([float(p) for p in position], dtype=torch.float64, device="cuda")[:, None, None] * inv.double()
+            low, high = heads[..., :half], heads[..., half:rot]
+            want[..., :half], want[..., half:rot] = low * angle.cos() - high * angle.sin(), high * angle.cos() + low * angle.sin()
+            size[..., :half] = size[..., half:rot] = low.abs() + high.abs()
+        else:
+            assert torch.equal(query, x[:, :q * hd]) and torch.equal(key, x[:, q * hd:(q + kv) * hd])
+        close_norm(query.view(rows, q, hd), want[:, :q], size[:, :q], dtype)
+        close_norm(key.view(rows, kv, hd), want[:, q:], size[:, q:], dtype)
+        values = x.view(rows, q + 2 * kv, hd)[:, q + kv:].float()
+        for r in range(rows):
+            for h in range(kv):
+                check_record(cache, sequence[r], slot[r], h, want[r, q + h], size[r, q + h], values[r, h])
+
+
 # ------------------------------------------------------------------------- the pages of the single-stream calls
 
 @pytest.mark.parametrize("enc", [F16, Q4H, Q8])
