@@ -457,7 +457,8 @@ int qllm_k_attention(uint32_t encoding, const uint8_t* const* page_table, size_t
  * cache is the one of the calls above (same pages, same records), one page table per sequence.
  *
  * All pointers are device memory of the current device unless stated, 4-byte aligned unless a call
- * asks for more (memory that is not the current device's is refused as far as the call can tell from qkv or page_tables);
+ * asks for more.  Memory of the host or of another device is refused as far as a call can tell from qkv, page_tables
+ * and its list of positions or lengths (lists may lie in pinned host memory);
  * the calls only enqueue on `stream`, allocate nothing, can be captured into a graph,
  * and keep nothing in the library, so calls on several streams and threads may run at once as long as
  * they share no workspace and no output.  Graphs that share a workspace must not run at once.
@@ -477,12 +478,13 @@ typedef struct qllm_kv_batch {
   uint32_t page_tokens, encoding;         /* QLLM_KV_* */
   uint32_t kv_heads, head_dim;
 } qllm_kv_batch;
-/* Per-head RMS norm of queries and keys, rotation by position, and the K/V records
- * (gated_gqa_qkv_rope_paged_batch_kernel with its per-head norm, transformer_kernels.cu:3551-3643,
- * for rows of many sequences).  Row r of qkv [rows, (q_heads + 2 kv_heads) * head_dim] (row_type values,
+/* Per-head RMS norm of queries and keys, rotation by position, and the K/V records, for rows of many sequences (the
+ * place of gated_gqa_qkv_rope_paged_batch_kernel, transformer_kernels.cu:3551-3643, with other conventions: that kernel's norm
+ * multiplies by 1 + weight, so q_norm and k_norm here are 1 + its stored weights, and its rows carry a gate beside each query
+ * head, which a host takes out first).  Row r of qkv [rows, (q_heads + 2 kv_heads) * head_dim] (row_type values,
  * qkv_stride elements apart):
  *   n = x * w / sqrt(mean(x^2) + eps) per query head (w = q_norm) and key head (w = k_norm), [head_dim] FP32; q_norm and
- *   k_norm both null: n = x, for models without a per-head norm;
+ *   k_norm both null: n = x, for models without a per-head norm; the squares are summed in FP32 and have to fit it;
  *   the first rotary_dim values (a multiple of 16, may be 0) are rotated in pairs (i, i + rotary_dim / 2)
  *   by positions[r] * inv_freq[i], the angle reduced in FP64;
  *   query [rows, q_heads * head_dim], and key [rows, kv_heads * head_dim] unless it is null, get the
@@ -497,7 +499,7 @@ typedef struct qllm_kv_batch {
  * slot_positions [sequences, kv_heads, slot_stride] (optional): positions[r] is written for each
  * head of the slot stored, which is what qllm_k_kv_evict reads.
  * Rows and strides in multiples of 16 bytes.  query may be qkv itself, and key its key heads, with the
- * same stride (in place). */
+ * same stride (in place); otherwise rows do not overlap, but may be columns of one buffer of one stride. */
 int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, const void* qkv, size_t qkv_stride,
                               uint32_t rows, uint32_t q_heads, uint32_t rotary_dim, const float* q_norm,
                               const float* k_norm, float eps, const float* inv_freq, const uint32_t* positions,
@@ -509,12 +511,15 @@ int qllm_k_qk_norm_rope_store(const qllm_kv_batch* cache, uint32_t row_type, con
  *   z_t = scale * q . K_t;  p = softmax(z);  out = sum_t p_t V_t        per query head
  *   weights_out[s, h, t] = weights_in[s, h, t] + sum of p_t over the query heads of kv head h
  * query, out [sequences, q_heads * head_dim] of row_type, rows and strides in multiples of 16 bytes, not
- * overlapping; scores, softmax statistics and sums are FP32, the result is rounded once.  A sequence of
+ * overlapping (they may be columns of one buffer); scores, softmax statistics and sums are FP32, the result is rounded once.
+ * What the products take: a query of 22 (F16 cache, FP32 rows) or 23 bits relative to its head's largest value (24 with
+ * FP32 rows over Q8 and Q4H; 16-bit rows over F16 as they are), and a weight p of 22 bits, 11 with BF16 rows.  Over Q8 and Q4H a
+ * key whose p times V scale is below 2^-10 of the largest has fewer of those bits, below 2^-32 none.  A sequence of
  * length 0 (or whose slots are all absent, or all score -inf) gives zeros.  A query head that holds a NaN or an
  * infinity gives NaN (BF16 and F16 rows over an F16 cache: what the formulas give).  weights_out
  * [sequences, kv_heads, weights_stride] is optional; weights_in null: zeros; weights_in == weights_out: in
  * place; slots at and behind lengths[s] are left alone.  workspace: at least
- * qllm_k_decode_attention_workspace_bytes bytes (0: a cache that the call refuses) on a 16-byte boundary, its content does
+ * qllm_k_decode_attention_workspace_bytes bytes (0: a cache or q_heads that the call refuses) on a 16-byte boundary, its content does
  * not matter. */
 size_t qllm_k_decode_attention_workspace_bytes(const qllm_kv_batch* cache, uint32_t q_heads, int weights);
 int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const void* query, size_t query_stride,
@@ -530,7 +535,9 @@ int qllm_k_decode_attention(const qllm_kv_batch* cache, uint32_t row_type, const
  * the records move in place and as few as possible.  weights_out and positions_out (== the inputs: in
  * place) hold the kept slots' values at t < m, weights_out is zero for m <= t < n (a slot stored there
  * later starts from nothing), everything else is left alone; lengths_out[s] = m (== lengths_in: in
- * place).  Slots on absent pages move no record; a page must not be in more than one sequence's table. */
+ * place: only where no other layer's call reads the same list, for each layer has its own weights and needs the
+ * lengths from before).  Slots on absent pages move no record; a page must not be in more than one place of the tables.
+ * The workspace size is 0 for a cache that the call refuses. */
 size_t qllm_k_kv_evict_workspace_bytes(const qllm_kv_batch* cache, uint32_t budget);
 int qllm_k_kv_evict(const qllm_kv_batch* cache, const uint32_t* lengths_in, uint32_t* lengths_out,
                     const uint32_t* next_positions, uint32_t budget, uint32_t recent, uint32_t sinks,

@@ -38,10 +38,11 @@
 // of a reduction), F16 holds them down to 2^-32 of the largest, and a key whose V is small has a small scale.
 //
 // Measured on one B200 (copy 6554 GB/s), device time of both launches: 64 sequences of up to 8192 tokens, F16, 32 query and 4 kv
-// heads of 128, BF16 rows: 100 us, 6.1 TB/s of cache, HBM-bound; 7 of up to 20001, F16, 16 heads of 64, FP32 rows, with weights:
-// 54 us, 4.4 TB/s (two terms a query and a weight: instruction issue, then the weights' pass); 96 of up to 4500, Q8, 40 and 8 heads
-// of 128, with weights: 133 us, 3.7 TB/s (unpacking bytes: instruction issue); 1 of 32768, Q4H, 40 and 8 heads of 128: 21 us,
-// 1.6 TB/s (a block's share is some 150 tokens a warp: set-up, merge and join are more than half); 1 of 1000, F16: 9.5 us (latency alone).
+// heads of 128, BF16 rows: 102 us, 6.1 TB/s of cache, HBM-bound; 7 of up to 20001, F16, 16 heads of 64, FP32 rows, with weights:
+// 58 us, 4.1 TB/s (two terms a query and a weight: instruction issue, then the weights' pass); 96 of up to 4500, Q8, 40 and 8 heads
+// of 128, F16 rows, with weights: 136 us, 3.6 TB/s, after a pause (unpacking bytes: instruction issue) and 143 to 154 us in calls one after
+// the other; 1 of 32768, Q4H, 40 and 8 heads of 128: 21 us, 1.6 TB/s (a block's share is some 150 tokens a warp: set-up, merge and join
+// are more than half); 1 of 1000, F16: 9.7 us (latency alone).
 #include <type_traits>
 
 #include "kernels.h"
@@ -1399,7 +1400,9 @@ int launch(const DecodeAttentionArgs& a, const Plan& plan, cudaStream_t stream) 
                   "decode_attention");
   if (rc) return rc;
   // The first launch does not call for the second early: blocks that wait beside it made 1 x 32768 Q4H 25.2 us instead of 23.6 us.
-  // Four warps to a query head as long as they find room at once.
+  // Four warps to a query head as long as they find room at once, up to eight heads to a multiprocessor (up to four: 34.3 -> 35.5 us for
+  // 16 x 8192 Q4H of 40 heads and 34.6 -> 36.0 for 32 x 4096 F16 of 32; up to sixteen: 89.4 -> 90.6 for 48 x 8192 Q4H and 60.5 -> 61.7 for
+  // 64 x 4096 F16, 70.0 -> 68.6 for 20 x 16384 Q8 of 64).
   const uint32_t heads = a.cache.sequences * a.q_heads;
   const uint32_t ways = heads <= 8U * sms ? kWarps : 1U;
   const uint32_t joins = ways == kWarps ? heads : (heads + kWarps - 1U) / kWarps;

@@ -32,7 +32,9 @@ namespace {
 constexpr uint32_t kSelectThreads = 512;
 constexpr uint32_t kSelectWarps = kSelectThreads / 32;
 constexpr uint32_t kBins = 2048;
-constexpr uint32_t kSlotsPerBlock = 4096;  // a row is spread over more blocks only above this
+// A row is spread over more blocks only above this (2048 / 4096 / 8192, 8 heads of 128: 1 of 4097 11.3 / 11.6 / 12.1 us, 1 of 8192 to half
+// 16.7 / 18.5 / 21.5, 4 of 8192 25.5 / 26.4 / 30.0, 1 of 16384 Q4H 20.1 / 19.0 / 23.4; 8 of 32768 and 48 of 6001 do not depend on it).
+constexpr uint32_t kSlotsPerBlock = 4096;
 constexpr uint32_t kMaxCluster = 8;
 constexpr uint32_t kAhead = 8;
 constexpr uint32_t kMaxKeys = 48U * 1024U;  // of one block in shared memory; longer rows read weights and positions again

@@ -18,7 +18,7 @@
 // while these are worked on.
 //
 // Measured on one B200 (copy 6554 GB/s): 8192 rows of 40 query and 8 kv heads of 128, BF16: 42 us for 235 MB, 0.85 of the copy
-// rate; 517 FP32 rows of 12 and 2 heads of 256: 8.5 us for 16.8 MB, the start of a launch and one chain of loads; 64 rows and one row:
+// rate (2048 rows: 14.7 us, 0.61; with Q8 or Q4H records 52 us; FP32 rows 109 us, 0.61); 517 FP32 rows of 12 and 2 heads of 256: 8.5 us for 16.8 MB, the start of a launch and one chain of loads; 64 rows and one row:
 // 4.1 and 3.6 us, a launch.
 #include "kv_batch.cuh"
 #include "launch.cuh"
@@ -28,7 +28,9 @@ namespace qllm {
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kWarpsWanted = 2048;  // of a launch (rows of 40 + 16 heads of 128: 2048: 9.4, 4096: 10.9, 8192: 12.9 us for 1024 rows)
+// Warps of a launch, for rows of 40 + 16 heads of 128 with 1024 / 2048 / 4096 of them: 512 rows 8.2 / 6.9 / 8.0 us, 1024 rows 11.3 / 9.3 / 10.8;
+// 1024 rows of 16 + 32 heads of 64: 7.5 / 6.2 / 7.1; from 2048 rows on, and for FP32 rows of 256, the same within 2 %.
+constexpr uint32_t kWarpsWanted = 2048;
 
 template <int kLanes>
 __device__ __forceinline__ float head_sum(float v) {
