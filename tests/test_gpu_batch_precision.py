@@ -108,15 +108,13 @@ def test_a_missing_term_would_show(q, kv, hd, enc, page):
     assert wrongly_rounded(got.half(), want) > WRONG[HF16]
 
 
-@pytest.mark.parametrize("dtype", [F32, BF16, HF16])
-@pytest.mark.parametrize("gap", [10.0, 14.0, 16.0, 20.0, 23.0, 40.0])
+# F16 rows: behind more than 14 nats the output is below F16's normal values
+@pytest.mark.parametrize("dtype,gap", [(t, g) for t in (F32, BF16, HF16) for g in (10.0, 14.0, 16.0, 20.0, 23.0, 40.0) if t != HF16 or g <= 14.0])
 @pytest.mark.parametrize("n", [40, 2048])
 def test_attention_behind_a_key_that_adds_nothing(dtype, gap, n):
     """An attention sink: one key scores `gap` nats above all others and its V is zero, so that the output is made of weights
     far below the largest.  An error of that key's score (8 e |z|) is one of every weight."""
     q, kv, hd, page = 8, 2, 128, 64
-    if dtype == HF16 and gap > 14.0:
-        pytest.skip("the output is below F16's normal values")
     cache = PagedCache(1, -(-n // page), page, F16, kv, hd, seed=5)
     both = cache.pool.view(HF16).view(-1, 2, page, kv, hd)
     if dtype == HF16:
