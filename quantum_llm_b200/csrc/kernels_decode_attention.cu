@@ -15,13 +15,13 @@
 // began before its share and one that goes on after it, hence two places per block -- and a second launch
 // joins those.  The split depends on the lengths alone, so the bits of a result do not depend on scheduling.
 //
-// Inner product on the tensor cores (mma.sync m16n8k16, F16 in, FP32 out) with the CACHE as the M operand:
+// Inner product on the tensor cores (mma.sync, FP32 out; operands below) with the CACHE as the M operand:
 // S^T = K q^T has 16 keys x 8 heads, out^T = V^T P^T 16 dims x 8 heads, so that a group of up to eight query
 // heads fills the N = 8 side instead of a sixteenth to a half of an M side.  tcgen05 wants an M of 64 or 128
 // and its operands in shared memory; here the keys go from global memory straight into the registers of a
 // fragment (no shared memory, no barrier) because the order of k inside a product is free: a lane takes
-// whichever 16 bytes of a row it can load at once, and the query is laid out to match.  For V^T the pairs
-// of keys that a fragment packs are put together by byte permutes.  Key 2 r stands in row r of a 16-key
+// whichever 16 bytes of a row it can load at once, and the query is laid out to match.  For V^T of Q8 and Q4H
+// the pairs of keys that a fragment packs are put together by byte permutes.  Key 2 r stands in row r of a 16-key
 // block, key 2 r + 1 in row r + 8, so that a lane's two keys (scales, scores) are neighbours.
 //
 // Numerics.  Codes of Q8 and Q4H records are small integers: K's meet the query as INT8 (mma.sync m16n8k32), the query as a

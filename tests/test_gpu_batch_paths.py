@@ -278,3 +278,61 @@ def test_norm_rope_store_of_many_passes(dtype, in_place, rot):
         assert torch.equal(x[~live], given[~live]) and torch.equal(x[:, (q + kv) * hd:], given[:, (q + kv) * hd:])
     else:
         assert torch.equal(x, given) and bool((query[~live] == 7).all()) and bool((key[~live] == 7).all())
+
+
+# ------------------------------------------------------------------------- several threads
+
+def test_calls_from_several_threads():
+    """Four threads, each with a stream, a cache and workspaces of its own, make the three calls at once; every thread's results are
+    those of the same calls made alone."""
+    import threading
+    q, kv, hd, page, sequences, budget, steps = 8, 2, 128, 16, 3, 60, 25
+    w, inv = 1 + 0.1 * rand(hd, 4), inv_freq(hd)
+
+    def run(i):
+        enc, dtype = (F16, Q4H, Q8, F16)[i], (BF16, HF16, F32, F32)[i]
+        cache = PagedCache(sequences, 8, page, enc, kv, hd, seed=i)
+        lengths, following = u32([50, 3, 59]), u32([50, 3, 59])
+        weights = torch.zeros(sequences, kv, 128, device="cuda")
+        positions = torch.arange(128, device="cuda", dtype=torch.int32).expand(sequences, kv, 128).clone()
+        rows = [rand((sequences, (q + 2 * kv) * hd), 10 * i + s).to(dtype) for s in range(steps)]
+        query = torch.zeros(sequences, q * hd, dtype=dtype, device="cuda")
+        outs = torch.zeros(steps, sequences, q * hd, dtype=dtype, device="cuda")
+        space, trim = bc.attention_workspace(cache, q, True), bc.evict_workspace(cache, budget)
+        torch.cuda.synchronize()
+
+        def go(barrier=None):
+            with torch.cuda.stream(torch.cuda.Stream()):
+                if barrier:
+                    barrier.wait(30)
+                for s in range(steps):
+                    bc.norm_rope_store(cache, rows[s], q, hd, w, w, inv, following, None, lengths, query, None, positions)
+                    lengths.add_(1)
+                    following.add_(1)
+                    bc.decode_attention(cache, query, lengths, q, hd ** -0.5, outs[s], weights, weights, space)
+                    bc.evict(cache, lengths, lengths, following, budget, 8, 2, weights, weights, positions, positions, trim)
+                torch.cuda.current_stream().synchronize()
+        return go, (cache.pool, lengths, weights, positions, outs)
+
+    alone = []
+    for i in range(4):
+        go, state = run(i)
+        go()
+        alone.append([t.clone() for t in state])
+    calls, failed, barrier = [run(i) for i in range(4)], [], threading.Barrier(4)
+
+    def work(go):
+        try:
+            go(barrier)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(go,)) for go, _ in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    torch.cuda.synchronize()
+    assert not failed and not any(t.is_alive() for t in threads)
+    for (_, state), want in zip(calls, alone):
+        assert all(torch.equal(bc.raw(a), bc.raw(b)) for a, b in zip(state, want))
